@@ -50,6 +50,9 @@
  *                     and the affine norm3 (wan/modules/causal_model.py:285-287)
  *   ss_rms_norm    <- WanRMSNorm (wan/modules/model.py:70-86) of the cross-attention query (:172)
  *   ss_gate_residual <- the gated residual adds (wan/modules/causal_model.py:337, 348-349)
+ *   ss_adaln_i8, ss_linear_i8 <- the same norms and the linear layers between them
+ *                     (wan/modules/causal_model.py:110-114, 328-349) in 8 bits; the reference
+ *                     quantises no linear layer
  */
 #ifndef SSPARSE_H_
 #define SSPARSE_H_
@@ -72,6 +75,11 @@ extern "C" {
 
 /* Devices per process the library keeps per-device state for (ordinals 0 .. 63). */
 #define SS_MAX_DEVICES 64
+
+/* element types of the 8-bit linear path's rows, biases and outputs */
+#define SS_BF16 0
+#define SS_F32 1
+#define SS_F16 2
 
 /* device-side status bits (OR-ed into *status) */
 #define SS_DEV_NONFINITE 0x1    /* a router score was NaN or +-inf */
@@ -513,6 +521,51 @@ int ss_rms_norm(const void *x, int64_t x_ld, int n, int d, const void *weight, f
  * NULL. y rows at stride y_ld elements. */
 int ss_gate_residual(void *x, const void *y, int64_t y_ld, int n, int d, int frame_tokens,
                      const float *gate, int64_t gate_ld, void *stream);
+
+/* ------------------------------------------------------------------------------------------ */
+/* 8-bit linear path: rows of 8-bit codes with one fp32 scale each, and their products.         */
+/*                                                                                              */
+/* A row x is held as codes q in [-127, 127] and a scale s with x ~= q * s, s = max|x| / 127 (at */
+/* least 1e-30, so a row of zeros has finite codes). A row that holds an infinity or a NaN gets  */
+/* codes 0 and scale NaN: its products are NaN, and no other row's are. Rows of every buffer may */
+/* lie at any stride (in elements, at least d); `dtype` is SS_BF16, SS_F32 or SS_F16 and holds   */
+/* for x, the residual, the norm's weight and bias, and the stored sum. n may be 0.              */
+/* ------------------------------------------------------------------------------------------ */
+
+/* q = rint(x * (1 / s)) for rows x [n][d] -> out [n][d] int8, scales [n]. */
+int ss_quant_rows(const void *x, int64_t x_ld, int dtype, int n, int d, int8_t *out,
+                  int64_t out_ld, float *scales, void *stream);
+
+/* Codes of v * rsqrt(mean(v^2) + eps) * weight, v = x + residual (residual may be NULL: v = x).
+ * `sum` (optional) gets v rounded to dtype; it may be x or residual itself. The norm reads v
+ * unrounded. The sum of squares is fp32: rows with values above about 1e18 overflow it and get
+ * scale 0. */
+int ss_rms_norm_i8(const void *x, int64_t x_ld, const void *residual, int64_t res_ld, int dtype,
+                   int n, int d, const void *weight, float eps, void *sum, int64_t sum_ld,
+                   int8_t *out, int64_t out_ld, float *scales, void *stream);
+
+/* Codes of LayerNorm(v), v = x + y * gate[f] (y NULL: v = x; gate NULL: v = x + y), followed by
+ * either the frame's modulation * (1 + scale[f]) + shift[f] or the affine * weight + bias (exactly
+ * one of the two forms); f = row / frame_tokens, shift and scale fp32 rows of stride mod_ld, gate
+ * fp32 rows of stride gate_ld. frame_tokens counts only where gate, shift or scale is given. `sum`
+ * as in ss_rms_norm_i8. */
+int ss_adaln_i8(const void *x, int64_t x_ld, const void *y, int64_t y_ld, const float *gate,
+                int64_t gate_ld, int dtype, int n, int d, int frame_tokens, const float *shift,
+                const float *scale, int64_t mod_ld, const void *weight, const void *bias, float eps,
+                void *sum, int64_t sum_ld, int8_t *out, int64_t out_ld, float *scales,
+                void *stream);
+
+/* The longest reduction of ss_linear_i8: 131071 products of 8-bit codes fit 32 bits. */
+#define SS_LINEAR_I8_MAX_K 131071
+
+/* out[m][n] = act(S * (xs[m] * ws[n]) + bias[n]), S = sum_k x[m][k] * w[n][k] exact in 32 bits; act
+ * is the tanh form of GELU where gelu != 0, else the identity. x [M][K] and w [N][K] int8, 16-byte
+ * aligned with row strides that are multiples of 16; bias [N] of bias_dtype or NULL; out [M][N] of
+ * out_dtype, row stride out_ld. `status` (optional) gets SS_DEV_TIMEOUT if a wait in the kernel ran
+ * out. M may be 0. */
+int ss_linear_i8(const int8_t *x, int64_t x_ld, const float *xs, const int8_t *w, int64_t w_ld,
+                 const float *ws, const void *bias, int bias_dtype, int gelu, int M, int N, int K,
+                 void *out, int64_t out_ld, int out_dtype, int *status, void *stream);
 
 #ifdef __cplusplus
 }

@@ -77,6 +77,11 @@ SIGNATURES = {
     "ss_adaln": ([_P, _I, _I, _I, _P, _P, _I64, _P, _P, _F, _P, _P], _I),
     "ss_rms_norm": ([_P, _I64, _I, _I, _P, _F, _P, _P], _I),
     "ss_gate_residual": ([_P, _P, _I64, _I, _I, _I, _P, _I64, _P], _I),
+    "ss_quant_rows": ([_P, _I64, _I, _I, _I, _P, _I64, _P, _P], _I),
+    "ss_rms_norm_i8": ([_P, _I64, _P, _I64, _I, _I, _I, _P, _F, _P, _I64, _P, _I64, _P, _P], _I),
+    "ss_adaln_i8": ([_P, _I64, _P, _I64, _P, _I64, _I, _I, _I, _I, _P, _P, _I64, _P, _P, _F, _P, _I64, _P, _I64, _P,
+                     _P], _I),
+    "ss_linear_i8": ([_P, _I64, _P, _P, _I64, _P, _P, _I, _I, _I, _I, _I, _P, _I64, _I, _P, _P], _I),
 }
 
 

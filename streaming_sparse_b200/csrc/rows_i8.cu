@@ -1,0 +1,217 @@
+// rows_i8.cu -- 8-bit rows with one scale each: the row quantiser and the norms that end in it.
+//
+//   ss_quant_rows   s = max(max|x| / 127, 1e-30);  q = rint(x * (1 / s))
+//   ss_rms_norm_i8  v = x + residual;  t = v * w;  u = max(max|t| / 127, 1e-30);
+//                   q = rint(t * (1 / u));  s = u * rsqrt(mean(v^2) + eps)
+//                   (the row's rsqrt is a common factor of its values, so it goes into the scale
+//                   and the codes need no statistic but the maximum: one pass gives both)
+//   ss_adaln_i8     v = x + y * gate[f];  z = (v - mean) * rsqrt(var + eps);
+//                   o = z * (1 + scale[f]) + shift[f]  or  z * w + b;
+//                   s = max(max|o| / 127, 1e-30);  q = rint(o * (1 / s))
+// The sum v is also stored, rounded once to the rows' type; the norm reads it unrounded. All
+// statistics are fp32. A row that holds an infinity or a NaN where its codes are made gets codes 0
+// and scale NaN, so that the products it enters are NaN and no other row's are.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace ss {
+namespace rows {
+
+constexpr float TINY = 1e-30f;   // the smallest scale: a row of zeros keeps a finite reciprocal
+
+enum Mode { QUANT, RMS, LN };
+
+struct Args {
+    const void *x;
+    int64_t x_ld;
+    const void *res;        // residual / y (null: none)
+    int64_t res_ld;
+    const float *gate;      // LN: per-frame gate rows (null: 1)
+    int64_t gate_ld;
+    const void *weight;     // RMS, affine LN
+    const void *bias;       // affine LN
+    const float *shift;     // modulated LN
+    const float *scale;
+    int64_t mod_ld;
+    void *sum;
+    int64_t sum_ld;
+    int8_t *out;
+    int64_t out_ld;
+    float *scales;
+    int n, d, frame_tokens;
+    float eps;
+};
+
+__device__ __forceinline__ float to_f(float v) { return v; }
+__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+__device__ __forceinline__ void from_f(float v, float &o) { o = v; }
+__device__ __forceinline__ void from_f(float v, __nv_bfloat16 &o) { o = __float2bfloat16_rn(v); }
+__device__ __forceinline__ void from_f(float v, __half &o) { o = __float2half_rn(v); }
+
+// |x| as an unsigned integer orders the finite numbers, then infinity, then the NaNs: one integer
+// maximum finds the largest magnitude and keeps what is not finite.
+__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+
+struct Scale {
+    float s, inv;
+};
+// the scale of a row from the largest magnitude's bits; codes rint(x * inv) are within +-127
+__device__ __forceinline__ Scale row_scale(uint32_t m) {
+    if (m >= 0x7f800000u) return {__uint_as_float(0x7fc00000u), 0.f};
+    const float s = fmaxf(__fdiv_rn(__uint_as_float(m), 127.f), TINY);
+    return {s, __frcp_rn(s)};
+}
+__device__ __forceinline__ int8_t code(float x, Scale s) {
+    return s.inv == 0.f ? (int8_t)0 : (int8_t)__float2int_rn(__fmul_rn(x, s.inv));
+}
+
+__device__ __forceinline__ float block_sum(float a, float *red) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = a;
+    __syncthreads();
+    float s = 0.f;
+    for (int i = 0; i < (int)(blockDim.x >> 5); ++i) s += red[i];   // the same order in every thread
+    return s;
+}
+__device__ __forceinline__ uint32_t block_max(uint32_t a, uint32_t *red) {
+    a = __reduce_max_sync(0xffffffffu, a);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = a;
+    __syncthreads();
+    uint32_t m = 0u;
+    for (int i = 0; i < (int)(blockDim.x >> 5); ++i) m = max(m, red[i]);
+    return m;
+}
+
+// One CTA per row, any width, stride and alignment: element loads, the row read once per statistic.
+template <typename T, int MODE>
+__global__ void __launch_bounds__(256) row_kernel(const Args p) {
+    __shared__ float fred[8];
+    __shared__ uint32_t ured[8];
+    const int64_t row = blockIdx.x;
+    const int t = threadIdx.x, d = p.d;
+    const T *x = static_cast<const T *>(p.x) + row * p.x_ld;
+    const T *r = p.res ? static_cast<const T *>(p.res) + row * p.res_ld : nullptr;
+    const int64_t f = (MODE == LN && p.frame_tokens > 0) ? row / p.frame_tokens : 0;
+    const float *g = p.gate ? p.gate + f * p.gate_ld : nullptr;
+    const T *w = static_cast<const T *>(p.weight), *b = static_cast<const T *>(p.bias);
+    const float *sh = p.shift + f * p.mod_ld, *sc = p.scale + f * p.mod_ld;
+    auto value = [&](int c) -> float {
+        float v = to_f(x[c]);
+        if (r) v = __fadd_rn(v, g ? __fmul_rn(to_f(r[c]), g[c]) : to_f(r[c]));
+        return v;
+    };
+    float mean = 0.f, rstd = 1.f;
+    if (MODE == RMS) {
+        float s = 0.f;
+        for (int c = t; c < d; c += blockDim.x) {
+            const float v = value(c);
+            s += v * v;
+        }
+        rstd = rsqrtf(__fadd_rn(__fdiv_rn(block_sum(s, fred), (float)d), p.eps));
+    } else if (MODE == LN) {
+        float s = 0.f;
+        for (int c = t; c < d; c += blockDim.x) s += value(c);
+        mean = __fdiv_rn(block_sum(s, fred), (float)d);
+        s = 0.f;
+        for (int c = t; c < d; c += blockDim.x) {
+            const float z = value(c) - mean;
+            s += z * z;
+        }
+        rstd = rsqrtf(__fadd_rn(__fdiv_rn(block_sum(s, fred), (float)d), p.eps));
+    }
+    auto coded = [&](int c, float v) -> float {   // what the codes stand for, up to RMS's rsqrt
+        if (MODE == QUANT) return v;
+        if (MODE == RMS) return __fmul_rn(v, to_f(w[c]));
+        const float z = (v - mean) * rstd;
+        return w ? z * to_f(w[c]) + to_f(b[c]) : z * (1.f + sc[c]) + sh[c];
+    };
+    uint32_t m = 0u;
+    for (int c = t; c < d; c += blockDim.x) m = max(m, abs_bits(coded(c, value(c))));
+    const Scale s = row_scale(block_max(m, ured));
+    for (int c = t; c < d; c += blockDim.x) {
+        const float v = value(c);
+        p.out[row * p.out_ld + c] = code(coded(c, v), s);
+        // after the last read of x[c] and r[c], by the thread that read them: the sum may be
+        // written over either
+        if (p.sum) from_f(v, static_cast<T *>(p.sum)[row * p.sum_ld + c]);
+    }
+    if (t == 0) p.scales[row] = MODE == RMS ? __fmul_rn(s.s, rstd) : s.s;
+}
+
+template <int MODE>
+static int launch(const Args &p, int dtype, cudaStream_t st) {
+    const unsigned threads = (unsigned)(p.d >= 256 ? 256 : (p.d + 31) / 32 * 32);
+    if (dtype == SS_BF16) row_kernel<__nv_bfloat16, MODE><<<p.n, threads, 0, st>>>(p);
+    else if (dtype == SS_F16) row_kernel<__half, MODE><<<p.n, threads, 0, st>>>(p);
+    else row_kernel<float, MODE><<<p.n, threads, 0, st>>>(p);
+    return (int)cudaGetLastError();
+}
+
+static size_t type_bytes(int dtype) { return dtype == SS_F32 ? 4 : 2; }
+static bool off(const void *p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) != 0; }
+
+// checks shared by the three entry points; 0 when the call is one the kernels can run
+static int check_rows(const Args &p, int dtype) {
+    if (dtype != SS_BF16 && dtype != SS_F32 && dtype != SS_F16) return SS_ERR_SHAPE;
+    if (p.n < 0 || p.d <= 0 || p.x_ld < p.d || p.out_ld < p.d) return SS_ERR_SHAPE;
+    if ((p.res && p.res_ld < p.d) || (p.sum && p.sum_ld < p.d)) return SS_ERR_SHAPE;
+    if (p.n == 0) return 0;   // buffers without rows may have no address
+    if (!p.x || !p.out || !p.scales) return SS_ERR_POINTER;
+    const size_t a = type_bytes(dtype);
+    if (off(p.x, a) || off(p.res, a) || off(p.sum, a) || off(p.weight, a) || off(p.bias, a) || off(p.scales, 4) ||
+        off(p.gate, 4) || off(p.shift, 4) || off(p.scale, 4))
+        return SS_ERR_POINTER;
+    return 0;
+}
+
+}  // namespace rows
+}  // namespace ss
+
+extern "C" int ss_quant_rows(const void *x, int64_t x_ld, int dtype, int n, int d, int8_t *out, int64_t out_ld,
+                             float *scales, void *stream) {
+    using namespace ss::rows;
+    Args p = {};
+    p.x = x, p.x_ld = x_ld, p.n = n, p.d = d, p.out = out, p.out_ld = out_ld, p.scales = scales;
+    const int rc = check_rows(p, dtype);
+    if (rc || n == 0) return rc;
+    return launch<QUANT>(p, dtype, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int ss_rms_norm_i8(const void *x, int64_t x_ld, const void *residual, int64_t res_ld, int dtype, int n,
+                              int d, const void *weight, float eps, void *sum, int64_t sum_ld, int8_t *out,
+                              int64_t out_ld, float *scales, void *stream) {
+    using namespace ss::rows;
+    Args p = {};
+    p.x = x, p.x_ld = x_ld, p.res = residual, p.res_ld = res_ld, p.weight = weight, p.eps = eps;
+    p.sum = sum, p.sum_ld = sum_ld, p.n = n, p.d = d, p.out = out, p.out_ld = out_ld, p.scales = scales;
+    if (!weight) return SS_ERR_POINTER;
+    const int rc = check_rows(p, dtype);
+    if (rc || n == 0) return rc;
+    return launch<RMS>(p, dtype, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int ss_adaln_i8(const void *x, int64_t x_ld, const void *y, int64_t y_ld, const float *gate,
+                           int64_t gate_ld, int dtype, int n, int d, int frame_tokens, const float *shift,
+                           const float *scale, int64_t mod_ld, const void *weight, const void *bias, float eps,
+                           void *sum, int64_t sum_ld, int8_t *out, int64_t out_ld, float *scales, void *stream) {
+    using namespace ss::rows;
+    Args p = {};
+    p.x = x, p.x_ld = x_ld, p.res = y, p.res_ld = y_ld, p.gate = gate, p.gate_ld = gate_ld;
+    p.shift = shift, p.scale = scale, p.mod_ld = mod_ld, p.weight = weight, p.bias = bias, p.eps = eps;
+    p.frame_tokens = frame_tokens, p.sum = sum, p.sum_ld = sum_ld, p.n = n, p.d = d;
+    p.out = out, p.out_ld = out_ld, p.scales = scales;
+    const bool affine = weight || bias, modulate = shift || scale;
+    if (affine == modulate) return SS_ERR_SHAPE;   // exactly one of the two forms
+    if ((affine && (!weight || !bias)) || (modulate && (!shift || !scale)) || (gate && !y)) return SS_ERR_POINTER;
+    if (((modulate || gate) && frame_tokens <= 0) || (modulate && mod_ld < d) || (gate && gate_ld < d))
+        return SS_ERR_SHAPE;
+    const int rc = check_rows(p, dtype);
+    if (rc || n == 0) return rc;
+    return launch<LN>(p, dtype, static_cast<cudaStream_t>(stream));
+}

@@ -842,11 +842,216 @@ def gate_residual(x: torch.Tensor, y: torch.Tensor, *, gate: torch.Tensor | None
     return x
 
 
+# ----------------------------------------------------------------------------------------------
+# 8-bit linear path (csrc/rows_i8.cu, csrc/linear_i8.cu): rows of int8 codes with one scale each
+# ----------------------------------------------------------------------------------------------
+_I8_TYPES = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}   # SS_BF16, SS_F32, SS_F16
+LINEAR_I8_MAX_K = 131071
+
+
+def _no_grad(*tensors) -> None:
+    if torch.is_grad_enabled():
+        for t in tensors:
+            _require(t is None or not t.requires_grad, "the 8-bit linear path has no gradient: call it under "
+                                                       "torch.no_grad() or detach its inputs")
+
+
+def _ld(t: torch.Tensor, name: str, n: int, d: int, dtype: torch.dtype, device) -> int:
+    """Row stride of t [n, d] (the values of a row contiguous, the rows at any stride of at least d)."""
+    if t.dtype != dtype or t.dim() != 2 or t.shape[0] != n or t.shape[1] != d or t.device != device:
+        raise ValueError(f"{name}: expected {dtype} [{n}, {d}] on {device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    ld, step = t.stride()
+    if n <= 1:
+        ld = -(-d // 16) * 16      # a single row has no stride
+    if (step != 1 and d != 1) or ld < d:
+        raise ValueError(f"{name}: rows of {d} contiguous values that do not overlap expected")
+    return ld
+
+
+def _vec(t: torch.Tensor, name: str, d: int, dtype: torch.dtype, device) -> int:
+    if t.dtype != dtype or t.numel() != d or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{name}: contiguous {dtype} [{d}] on {device} expected")
+    return t.data_ptr()
+
+
+def _frame_rows(t: torch.Tensor, name: str, n: int, d: int, frame_tokens: int, device) -> int:
+    if t.dtype != torch.float32 or t.dim() != 2 or t.shape[1] != d or t.device != device:
+        raise ValueError(f"{name}: fp32 [frames, {d}] on {device} expected")
+    if frame_tokens <= 0 or t.shape[0] * frame_tokens < n:
+        raise ValueError("frame_tokens must cover the rows")
+    ld, step = t.stride()
+    if t.shape[0] <= 1:
+        ld = d
+    if (step != 1 and d != 1) or ld < d:
+        raise ValueError(f"{name}: rows of {d} contiguous values that do not overlap expected")
+    return ld
+
+
+def rows_i8(n: int, d: int, device) -> torch.Tensor:
+    """An uninitialised int8 [n, d] whose rows start at multiples of 16 bytes, as ``linear_i8`` reads them."""
+    if d % 16 == 0:
+        return torch.empty((n, d), dtype=torch.int8, device=device)
+    return torch.empty((n, -(-d // 16) * 16), dtype=torch.int8, device=device)[:, :d]
+
+
+def _rows_i8_in(x: torch.Tensor, name: str):
+    if not x.is_cuda or x.dim() != 2 or x.dtype not in _I8_TYPES or x.shape[1] < 1:
+        raise ValueError(f"{name}: CUDA tensor [n, d >= 1] of bfloat16, float16 or float32 expected")
+    return x.shape[0], x.shape[1], x.dtype, x.device
+
+
+def _rows_i8_out(out, scales, n: int, d: int, device):
+    if out is None:
+        out, ld = rows_i8(n, d, device), -(-d // 16) * 16
+    else:
+        ld = _ld(out, "out", n, d, torch.int8, device)
+    if scales is None:
+        scales = torch.empty(n, dtype=torch.float32, device=device)
+    else:
+        _vec(scales, "scales", n, torch.float32, device)
+    return out, ld, scales
+
+
+def quant_rows(x: torch.Tensor, *, out: torch.Tensor | None = None, scales: torch.Tensor | None = None):
+    """8-bit rows of x [n, d] bf16, fp16 or fp32 (any row stride): (x_i8 [n, d] int8, scales [n] fp32).
+
+    scale = max(max|x| / 127, 1e-30) and x_i8 = rint(x * (1 / scale)) per row, so x ~= x_i8 * scale
+    (`ss_quant_rows`). A row that holds an infinity or a NaN gets codes 0 and scale NaN. On a linear
+    layer's weight [N, K] it gives one scale for each output channel, as ``linear_i8`` wants it.
+    """
+    n, d, dtype, dev = _rows_i8_in(x, "x")
+    _no_grad(x)
+    x_ld = _ld(x, "x", n, d, dtype, dev)
+    out, o_ld, scales = _rows_i8_out(out, scales, n, d, dev)
+    rc = lib().ss_quant_rows(x.data_ptr(), x_ld, _I8_TYPES[dtype], n, d, out.data_ptr(), o_ld, scales.data_ptr(),
+                             _stream(dev))
+    check(rc, "ss_quant_rows")
+    return out, scales
+
+
+def rms_norm_i8(x: torch.Tensor, weight: torch.Tensor, eps: float, *, residual: torch.Tensor | None = None,
+                sum_out: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                scales: torch.Tensor | None = None):
+    """RMSNorm of x (+ residual) with 8-bit rows out (`ss_rms_norm_i8`).
+
+    x [n, d] bf16, fp16 or fp32 (any row stride), residual like it, weight [d] of the same type.
+    v = x + residual in fp32; (x_i8, scales) are the 8-bit rows of v * rsqrt(mean(v^2) + eps) * weight.
+    With a residual the sum v, rounded to x's type, is returned third; ``sum_out`` (x or residual
+    themselves, or another buffer) receives it. Non-finite rows as in ``quant_rows``.
+    """
+    n, d, dtype, dev = _rows_i8_in(x, "x")
+    _no_grad(x, weight, residual)
+    x_ld = _ld(x, "x", n, d, dtype, dev)
+    w = _vec(weight, "weight", d, dtype, dev)
+    r, r_ld, s, s_ld = _residual(residual, sum_out, "residual", n, d, dtype, dev)
+    out, o_ld, scales = _rows_i8_out(out, scales, n, d, dev)
+    rc = lib().ss_rms_norm_i8(x.data_ptr(), x_ld, r, r_ld, _I8_TYPES[dtype], n, d, w, float(eps),
+                              None if s is None else s.data_ptr(), s_ld, out.data_ptr(), o_ld, scales.data_ptr(),
+                              _stream(dev))
+    check(rc, "ss_rms_norm_i8")
+    return (out, scales) if s is None else (out, scales, s)
+
+
+def _residual(residual, sum_out, name: str, n: int, d: int, dtype, dev):
+    """(residual pointer, its row stride, sum buffer, its row stride); the sum goes with a residual."""
+    if residual is None:
+        _require(sum_out is None, f"sum_out goes with {name}")
+        return None, 0, None, 0
+    r_ld = _ld(residual, name, n, d, dtype, dev)
+    if sum_out is None:
+        return residual.data_ptr(), r_ld, torch.empty((n, d), dtype=dtype, device=dev), d
+    return residual.data_ptr(), r_ld, sum_out, _ld(sum_out, "sum_out", n, d, dtype, dev)
+
+
+def adaln_i8(x: torch.Tensor, *, eps: float, shift: torch.Tensor | None = None, scale: torch.Tensor | None = None,
+             frame_tokens: int = 0, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
+             y: torch.Tensor | None = None, gate: torch.Tensor | None = None, sum_out: torch.Tensor | None = None,
+             out: torch.Tensor | None = None, scales: torch.Tensor | None = None):
+    """LayerNorm of x (+ y * gate) with modulation or affine, 8-bit rows out (`ss_adaln_i8`).
+
+    x [n, d] bf16, fp16 or fp32 (any row stride), y like it. v = x + y * gate[f] in fp32 (gate fp32
+    [frames, d], absent: 1), f = row // frame_tokens; (x_i8, scales) are the 8-bit rows of
+    LayerNorm(v) * (1 + scale[f]) + shift[f] (fp32 [frames, d], any row stride), or of
+    LayerNorm(v) * weight + bias (both [d] of x's type). With y the sum v, rounded to x's type, is
+    returned third; ``sum_out`` (x or y themselves, or another buffer) receives it.
+    """
+    n, d, dtype, dev = _rows_i8_in(x, "x")
+    _no_grad(x, shift, scale, weight, bias, y, gate)
+    x_ld = _ld(x, "x", n, d, dtype, dev)
+    m = [None, None, None, None]
+    mod_ld = g_ld = 0
+    if weight is not None or bias is not None:
+        _require(weight is not None and bias is not None, "weight and bias go together")
+        _require(shift is None and scale is None, "give shift and scale, or weight and bias")
+        m[2], m[3] = _vec(weight, "weight", d, dtype, dev), _vec(bias, "bias", d, dtype, dev)
+    else:
+        _require(shift is not None and scale is not None, "give shift and scale, or weight and bias")
+        mod_ld = _frame_rows(shift, "shift", n, d, frame_tokens, dev)
+        _require(_frame_rows(scale, "scale", n, d, frame_tokens, dev) == mod_ld,
+                 "shift and scale must share a row stride")
+        m[0], m[1] = shift.data_ptr(), scale.data_ptr()
+    if gate is not None:
+        _require(y is not None, "gate goes with y")
+        g_ld = _frame_rows(gate, "gate", n, d, frame_tokens, dev)
+    r, r_ld, s, s_ld = _residual(y, sum_out, "y", n, d, dtype, dev)
+    out, o_ld, scales = _rows_i8_out(out, scales, n, d, dev)
+    rc = lib().ss_adaln_i8(x.data_ptr(), x_ld, r, r_ld, None if gate is None else gate.data_ptr(), g_ld,
+                           _I8_TYPES[dtype], n, d, int(frame_tokens), m[0], m[1], mod_ld, m[2], m[3], float(eps),
+                           None if s is None else s.data_ptr(), s_ld, out.data_ptr(), o_ld, scales.data_ptr(),
+                           _stream(dev))
+    check(rc, "ss_adaln_i8")
+    return (out, scales) if s is None else (out, scales, s)
+
+
+def linear_i8(x_i8: torch.Tensor, xs: torch.Tensor, w_i8: torch.Tensor, ws: torch.Tensor, *,
+              bias: torch.Tensor | None = None, gelu: bool = False, out_dtype: torch.dtype = torch.bfloat16,
+              out: torch.Tensor | None = None, validate: bool = False) -> torch.Tensor:
+    """The linear layer on 8-bit rows: act((x_i8 @ w_i8^T) * xs[:, None] * ws + bias) (`ss_linear_i8`).
+
+    x_i8 [M, K] and w_i8 [N, K] int8 with rows at multiples of 16 bytes (``rows_i8``; what
+    ``quant_rows``, ``rms_norm_i8`` and ``adaln_i8`` return), xs [M] and ws [N] fp32 scales, bias [N]
+    bf16, fp16 or fp32, ``gelu`` the tanh form of GELU. The products are summed exactly in 32-bit
+    integers (K <= 131071), scaled in fp32 and rounded once to ``out_dtype`` [M, N]. A row whose
+    scale is NaN gives a row of NaN.
+    """
+    if not x_i8.is_cuda or x_i8.dim() != 2 or w_i8.dim() != 2:
+        raise ValueError("x_i8 and w_i8: CUDA tensors [M, K] and [N, K] expected")
+    M, K = x_i8.shape
+    N, dev = w_i8.shape[0], x_i8.device
+    if N < 1 or not 1 <= K <= LINEAR_I8_MAX_K:
+        raise ValueError(f"N >= 1 and 1 <= K <= {LINEAR_I8_MAX_K} expected, got N = {N}, K = {K}")
+    _no_grad(xs, ws, bias)
+    x_ld, w_ld = _ld(x_i8, "x_i8", M, K, torch.int8, dev), _ld(w_i8, "w_i8", N, K, torch.int8, dev)
+    xp, wp = x_i8.data_ptr(), w_i8.data_ptr()
+    if (x_ld | w_ld | xp | wp) % 16:
+        raise ValueError("x_i8 and w_i8: rows must start at multiples of 16 bytes (ops.rows_i8 lays them out)")
+    xsp, wsp = _vec(xs, "xs", M, torch.float32, dev), _vec(ws, "ws", N, torch.float32, dev)
+    if bias is not None and bias.dtype not in _I8_TYPES:
+        raise ValueError("bias: bfloat16, float16 or float32 expected")
+    bp = None if bias is None else _vec(bias, "bias", N, bias.dtype, dev)
+    if out is None:
+        if out_dtype not in _I8_TYPES:
+            raise ValueError("out_dtype: bfloat16, float16 or float32 expected")
+        out, o_ld = torch.empty((M, N), dtype=out_dtype, device=dev), N
+    else:
+        _require(out.dtype in _I8_TYPES, "out: bfloat16, float16 or float32 expected")
+        o_ld = _ld(out, "out", M, N, out.dtype, dev)
+    status = DeviceStatus.word(dev)
+    rc = lib().ss_linear_i8(xp, x_ld, xsp, wp, w_ld, wsp, bp, 0 if bias is None else _I8_TYPES[bias.dtype],
+                            int(gelu), M, N, K, out.data_ptr(), o_ld, _I8_TYPES[out.dtype], status.data_ptr(),
+                            _stream(dev))
+    check(rc, "ss_linear_i8")
+    if validate:
+        DeviceStatus.check(dev)
+    return out
+
+
 __all__ = ["Workspace", "DeviceStatus", "route", "router_workspace_bytes", "RouterKeys", "pool_keys",
            "history_blocks", "sparse_attention", "sparse_attention_heads", "exact",
            "attention_max_ids", "attention_workspace_bytes", "lse_merge", "merge", "cache_append", "budget", "forced_count", "nblocks",
            "Ring", "cache_append_ring", "ring_refresh", "qkv_norm_rope_ring", "ring_commit",
-           "rope_shift", "qkv_norm_rope", "adaln", "rms_norm", "gate_residual"]
+           "rope_shift", "qkv_norm_rope", "adaln", "rms_norm", "gate_residual",
+           "rows_i8", "quant_rows", "rms_norm_i8", "adaln_i8", "linear_i8"]
 
 # keep the status-bit names importable from here
 DEV_BITS = dict(nonfinite=DEV_NONFINITE, timeout=DEV_TIMEOUT, badid=DEV_BADID)

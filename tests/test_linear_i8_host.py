@@ -1,0 +1,63 @@
+"""The 8-bit linear path without a GPU: what its entry points refuse on the host, and the row layout."""
+import ctypes
+
+import pytest
+import torch
+
+from streaming_sparse_b200 import ops
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from streaming_sparse_b200 import build
+    build.build()
+    from streaming_sparse_b200._lib import lib as load
+    return load()
+
+
+def test_host_argument_errors(lib):
+    fake = ctypes.c_void_p(0x100000)  # never dereferenced: every call fails its host checks, or has no rows
+    odd = ctypes.c_void_p(0x100002)
+    q = lib.ss_quant_rows
+    assert q(fake, 64, 0, 0, 64, fake, 64, fake, None) == 0
+    assert q(fake, 63, 0, 4, 64, fake, 64, fake, None) == 1001      # rows overlap
+    assert q(fake, 64, 3, 4, 64, fake, 64, fake, None) == 1001      # no such type
+    assert q(fake, 64, 0, 4, 0, fake, 64, fake, None) == 1001
+    assert q(None, 64, 0, 4, 64, fake, 64, fake, None) == 1002
+    assert q(odd, 64, 1, 4, 64, fake, 64, fake, None) == 1002       # fp32 off 4 bytes
+    r = lib.ss_rms_norm_i8
+    assert r(fake, 64, None, 0, 0, 0, 64, fake, 1e-6, None, 0, fake, 64, fake, None) == 0
+    assert r(fake, 64, None, 0, 0, 4, 64, None, 1e-6, None, 0, fake, 64, fake, None) == 1002
+    assert r(fake, 64, fake, 32, 0, 4, 64, fake, 1e-6, None, 0, fake, 64, fake, None) == 1001
+    a = lib.ss_adaln_i8
+    tail = (1e-6, None, 0, fake, 64, fake, None)
+    assert a(fake, 64, None, 0, None, 0, 0, 0, 64, 4, fake, fake, 64, None, None, *tail) == 0
+    assert a(fake, 64, None, 0, None, 0, 0, 4, 64, 4, None, None, 0, None, None, *tail) == 1001   # neither form
+    assert a(fake, 64, None, 0, None, 0, 0, 4, 64, 4, fake, fake, 64, fake, fake, *tail) == 1001  # both
+    assert a(fake, 64, None, 0, None, 0, 0, 4, 64, 0, fake, fake, 64, None, None, *tail) == 1001  # no frame size
+    assert a(fake, 64, None, 0, fake, 64, 0, 4, 64, 4, fake, fake, 64, None, None, *tail) == 1002  # a gate without y
+    assert a(fake, 64, None, 0, None, 0, 0, 4, 64, 4, fake, None, 64, None, None, *tail) == 1002
+    g = lib.ss_linear_i8
+    assert g(fake, 64, fake, fake, 64, fake, None, 0, 0, 0, 8, 64, fake, 8, 0, None, None) == 0
+    assert g(fake, 64, fake, fake, 64, fake, None, 0, 0, 4, 0, 64, fake, 8, 0, None, None) == 1001
+    assert g(fake, 72, fake, fake, 64, fake, None, 0, 0, 4, 8, 64, fake, 8, 0, None, None) == 1001   # stride off 16
+    assert g(fake, 131072, fake, fake, 131072, fake, None, 0, 0, 4, 8, 131072, fake, 8, 0, None, None) == 1001
+    assert g(fake, 64, fake, fake, 64, fake, fake, 3, 0, 4, 8, 64, fake, 8, 0, None, None) == 1001
+    assert g(odd, 64, fake, fake, 64, fake, None, 0, 0, 4, 8, 64, fake, 8, 0, None, None) == 1002
+    assert g(fake, 64, fake, fake, 64, None, None, 0, 0, 4, 8, 64, fake, 8, 0, None, None) == 1002
+    assert g(fake, 64, fake, fake, 64, fake, None, 0, 0, 4, 8, 64, odd, 8, 1, None, None) == 1002
+
+
+def test_host_tensors_are_refused():
+    x = torch.zeros(4, 64, dtype=torch.bfloat16)
+    q, s = torch.zeros(4, 64, dtype=torch.int8), torch.zeros(4)
+    for call in (lambda: ops.quant_rows(x), lambda: ops.rms_norm_i8(x, x[0], 1e-6),
+                 lambda: ops.adaln_i8(x, eps=1e-6, weight=x[0], bias=x[0]), lambda: ops.linear_i8(q, s, q, s)):
+        with pytest.raises(ValueError):
+            call()
+
+
+def test_rows_i8_start_at_multiples_of_16_bytes():
+    for d in (1, 15, 16, 17, 1536, 1549):
+        t = ops.rows_i8(3, d, "cpu")
+        assert t.shape == (3, d) and t.stride(1) == 1 and t.stride(0) % 16 == 0 and t.stride(0) >= d
