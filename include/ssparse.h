@@ -557,6 +557,8 @@ int ss_adaln_i8(const void *x, int64_t x_ld, const void *y, int64_t y_ld, const 
 
 /* The longest reduction of ss_linear_i8: 131071 products of 8-bit codes fit 32 bits. */
 #define SS_LINEAR_I8_MAX_K 131071
+/* The most rows of x, and of w, in one call. */
+#define SS_LINEAR_I8_MAX_ROWS 2147480000
 
 /* out[m][n] = act(S * (xs[m] * ws[n]) + bias[n]), S = sum_k x[m][k] * w[n][k] exact in 32 bits; act
  * is the tanh form of GELU where gelu != 0, else the identity. x [M][K] and w [N][K] int8, 16-byte

@@ -8,6 +8,7 @@ namespace ss {
 int attention_prepare(int device);
 int router_prepare(int device);
 int attention_i8_prepare(int device);
+int linear_i8_prepare(int device);
 
 using EncodeTiledFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
                                    const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
@@ -99,6 +100,8 @@ extern "C" int ss_prepare_device(void) {
     int rc = ss::attention_prepare(device);
     if (rc) return rc;
     rc = ss::attention_i8_prepare(device);
+    if (rc) return rc;
+    rc = ss::linear_i8_prepare(device);
     if (rc) return rc;
     return ss::router_prepare(device);
 }
