@@ -22,7 +22,7 @@ namespace lin {
 struct Params {
     const float *xs, *ws;
     const void *bias;
-    int bias_dtype, gelu, out_dtype;
+    int bias_dtype;
     int M, N, K;
     void *out;
     int64_t out_ld;
@@ -30,7 +30,7 @@ struct Params {
     int tn;      // tokens a tile
     int ncb;     // channel blocks
     int ntiles;  // channel blocks x token blocks (pairs)
-    int vec;     // rows of out take 4-channel vector stores
+    int vec;     // rows of out take 16-byte stores (pairs), 4-channel stores (split)
 };
 
 __device__ __forceinline__ float load_any(const void *p, int dtype, int64_t i) {
@@ -45,16 +45,39 @@ __device__ __forceinline__ void store_one(void *p, int64_t i, float v) {
     else static_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(v);
 }
 
-// tanh form of GELU, 0.5 v (1 + tanh(u)) = v / (1 + exp(-2u)), u = sqrt(2/pi) (v + 0.044715 v^3):
-// no cancellation for negative v, and an exponential that overflows gives -0
-__device__ __forceinline__ float gelu_tanh(float v) {
-    const float u2 = 1.5957691216057308f * v * (1.f + 0.044715f * v * v);
-    return v / (1.f + __expf(-u2));
+// two fp32 values in one 64-bit register (mul, add and fma as two IEEE operations each)
+__device__ __forceinline__ uint64_t f2(float lo, float hi) {
+    return ((uint64_t)__float_as_uint(hi) << 32) | __float_as_uint(lo);
 }
-__device__ __forceinline__ float finish(int acc, float s, float b, bool has_bias, bool gelu) {
-    float v = __fmul_rn((float)acc, s);
-    if (has_bias) v = __fadd_rn(v, b);
-    return gelu ? gelu_tanh(v) : v;
+__device__ __forceinline__ float f2_lo(uint64_t x) { return __uint_as_float((uint32_t)x); }
+__device__ __forceinline__ float f2_hi(uint64_t x) { return __uint_as_float((uint32_t)(x >> 32)); }
+__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ float rcp(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Two finished values: act(float(acc) * s + b). The tanh form of GELU is computed as
+// 0.5 v (1 + tanh(u)) = v / (1 + exp(-2u)), u = sqrt(2/pi) (v + 0.044715 v^3): no cancellation for
+// negative v, and an exponential that overflows gives -0. The exponential is 2^(-2u log2(e)).
+template <bool GELU>
+__device__ __forceinline__ uint64_t finish(int acc0, int acc1, uint64_t s, uint64_t b) {
+    const uint64_t v = f2_fma(f2((float)acc0, (float)acc1), s, b);
+    if (!GELU) return v;
+    constexpr float A = -2.302208198144325f;             // -2 sqrt(2/pi) log2(e)
+    constexpr float B = A * 0.044715f;
+    const uint64_t t = f2_mul(v, f2_fma(f2_mul(v, v), f2(B, B), f2(A, A)));
+    return f2_mul(v, f2(rcp(1.f + ex2(f2_lo(t))), rcp(1.f + ex2(f2_hi(t)))));
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -105,6 +128,26 @@ __device__ __forceinline__ void mma_i8(uint32_t d_tmem, uint64_t a_desc, uint64_
             ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
             : "memory");
 }
+// 16 TMEM lanes x 32 columns as four 8-column fragments: v[4 i + 2 e + t] is lane 8 e + l / 4 (l this
+// thread's lane in the warp), column 8 i + 2 (l % 4) + t
+__device__ __forceinline__ void tmem_ld_16x256b_x4(uint32_t taddr, float *v) {
+    uint32_t *r = reinterpret_cast<uint32_t *>(v);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+// two values rounded to 16 bits, the first in the low half
+template <int DT>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    if (DT == SS_F16) {
+        const __half2 h = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+    return pack_bf16x2(lo, hi);
+}
 // signals the barrier at this place in both CTAs of the pair once the MMAs issued so far are done
 __device__ __forceinline__ void commit_both(uint32_t bar) {
     asm volatile(
@@ -145,19 +188,21 @@ constexpr int EPI_WARPS = 8;
 constexpr int THREADS = (EPI_WARPS + 2) * 32;
 constexpr uint32_t X_BYTES = 128 * BK;           // half of 256 tokens
 constexpr uint32_t STAGE_BYTES = W_BYTES + X_BYTES;
-constexpr uint32_t OFF_BAR = STAGES * STAGE_BYTES;
+constexpr uint32_t OFF_TURN = STAGES * STAGE_BYTES;            // per epilogue warp: 32 tokens x 32 channels of 16 bits
+constexpr uint32_t OFF_BAR = OFF_TURN + EPI_WARPS * 2048;
 enum Bar { FULL = 0, EMPTY = FULL + STAGES, ACC_FULL = EMPTY + STAGES, ACC_EMPTY = ACC_FULL + 2,
            DRAIN = ACC_EMPTY + 2, NBAR = DRAIN + 1 };
 constexpr uint32_t OFF_MISC = OFF_BAR + NBAR * 8 + (NBAR % 2) * 8;   // [0] tmem, [1] abort
 constexpr uint32_t OFF_XS = OFF_MISC + 16;
 constexpr uint32_t SMEM_BYTES = OFF_XS + EPI_WARPS * 32 * 4 + 1024;         // + alignment slack
 
-template <int DT>
+template <int DT, bool GELU>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, const Params p) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const uint32_t sbase = smem_u32(smem);
+    constexpr int NCH = DT == SS_F32 ? 1 : 4;   // channels a thread
     auto bar = [&](int i) -> uint32_t { return sbase + OFF_BAR + 8u * (uint32_t)i; };
     volatile uint32_t *misc = reinterpret_cast<volatile uint32_t *>(smem + OFF_MISC);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + OFF_MISC + 4);
@@ -186,37 +231,101 @@ kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtenso
     const uint32_t tmem = misc[0];
 
     if (warp < EPI_WARPS) {
-        // ---------------- epilogue: one channel per thread, every other 32 tokens ----------------
+        // ---------------- epilogue: 32 channels per warp, every other 32 tokens of the tile ----------------
         const int wg = warp >> 2;
         const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
         const uint32_t acc_empty = in_cta(bar(ACC_EMPTY), 0);
-        float *xs_s = reinterpret_cast<float *>(smem + OFF_XS) + warp * 32;   // the warp's 32 token scales
+        float *xs_s = reinterpret_cast<float *>(smem + OFF_XS) + warp * 32;   // the chunk's token scales
+        const uint32_t turn = sbase + OFF_TURN + (uint32_t)warp * 2048;
         bool ok = true;
         int it = 0;
         for (int tile = pair_id; tile < p.ntiles && ok; tile += npairs, ++it) {
-            const int n = (tile % p.ncb) * 256 + (int)rank * 128 + 32 * (warp & 3) + lane;
+            const int nw = (tile % p.ncb) * 256 + (int)rank * 128 + 32 * (warp & 3);   // the warp's channels
             const int64_t m0 = (int64_t)(tile / p.ncb) * p.tn;
-            const float wsv = n < p.N ? p.ws[n] : 0.f;
-            const float bv = (p.bias && n < p.N) ? load_any(p.bias, p.bias_dtype, n) : 0.f;
+            // the channels this thread gets of an accumulator: lane (32-bit output), or lane / 4 + 8 i
+            float wsv[NCH], bv[NCH];
+#pragma unroll
+            for (int i = 0; i < NCH; ++i) {
+                const int n = nw + (DT == SS_F32 ? lane : (lane >> 2) + 8 * i);
+                wsv[i] = n < p.N ? p.ws[n] : 0.f;
+                bv[i] = (p.bias && n < p.N) ? load_any(p.bias, p.bias_dtype, n) : 0.f;
+            }
             const int b = it & 1;
             ok = warp_all(mbar_wait(bar(ACC_FULL + b), (it >> 1) & 1, abort_flag));
             if (!ok) break;
             tc_fence_after();
             for (int c = wg; c < p.tn / 32; c += 2) {
-                float v[32];
-                tmem_ld32(lanes + 256 * b + 32 * c, v);
                 const int64_t mc = m0 + 32 * c;
-                __syncwarp();   // the chunk before has been read
-                xs_s[lane] = mc + lane < p.M ? p.xs[mc + lane] : 0.f;
+                const int rows = (int)min((int64_t)32, p.M - mc);
+                float v[32];
+                if (DT == SS_F32) {
+                    tmem_ld32(lanes + 256 * b + 32 * c, v);
+                } else {   // 16 channels x 32 tokens twice, as 8 x 8 fragments
+                    tmem_ld_16x256b_x4(lanes + 256 * b + 32 * c, v);
+                    tmem_ld_16x256b_x4(lanes + 256 * b + 32 * c + (16u << 16), v + 16);
+                }
+                __syncwarp();   // the chunk before has left the warp's shared memory
+                xs_s[lane] = lane < rows ? p.xs[mc + lane] : 0.f;
                 __syncwarp();
                 tmem_wait_ld();
                 tmem_ld_fence32(v);
-                const int rows = (int)min((int64_t)32, p.M - mc);
+                if constexpr (DT == SS_F32) {
+                    // thread = channel: a warp store covers 32 channels of a token, 128 bytes
 #pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                    const float y = finish(__float_as_int(v[j]), __fmul_rn(xs_s[j], wsv), bv,
-                                           p.bias != nullptr, p.gelu != 0);
-                    if (j < rows && n < p.N) store_one<DT>(p.out, (mc + j) * p.out_ld + n, y);
+                    for (int j = 0; j < 32; j += 2) {
+                        const uint64_t y = finish<GELU>(__float_as_int(v[j]), __float_as_int(v[j + 1]),
+                                                        f2_mul(f2(xs_s[j], xs_s[j + 1]), f2(wsv[0], wsv[0])),
+                                                        f2(bv[0], bv[0]));
+                        if (nw + lane < p.N) {
+                            float *dst = static_cast<float *>(p.out) + (mc + j) * p.out_ld + nw + lane;
+                            if (j < rows) dst[0] = f2_lo(y);
+                            if (j + 1 < rows) dst[p.out_ld] = f2_hi(y);
+                        }
+                    }
+                } else {
+                // v[16 h + 4 i + 2 e + t]: channel 16 h + 8 e + lane / 4, token 8 i + 2 (lane % 4) + t
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float2 x2 = *reinterpret_cast<const float2 *>(xs_s + 8 * i + 2 * (lane & 3));
+                    const uint64_t xs2 = f2(x2.x, x2.y);
+                    uint32_t o[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int at = 16 * (e >> 1) + 4 * i + 2 * (e & 1);
+                        const uint64_t y = finish<GELU>(__float_as_int(v[at]), __float_as_int(v[at + 1]),
+                                                        f2_mul(xs2, f2(wsv[e % NCH], wsv[e % NCH])),
+                                                        f2(bv[e % NCH], bv[e % NCH]));
+                        o[e] = pack2<DT>(f2_lo(y), f2_hi(y));
+                    }
+                    // transposed into rows of 32 channels: matrix e of the store is channels 8 e .. 8 e + 7 of
+                    // tokens 8 i .. 8 i + 7, lane l gives the row of token 8 i + l % 8 of matrix l / 8
+                    const int tok = 8 * i + (lane & 7);
+                    const uint32_t to = turn + (uint32_t)(tok * 64 + (((lane >> 3) ^ ((tok >> 1) & 3)) << 4));
+                    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};"
+                                 ::"r"(to), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]) : "memory");
+                }
+                __syncwarp();
+                // lane l: channels 8 (l % 4) .. + 8 of tokens l / 4 + 8 i
+                const int nc = nw + 8 * (lane & 3);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int tok = 8 * i + (lane >> 2);
+                    const uint32_t from = turn + (uint32_t)(tok * 64 + (((lane & 3) ^ ((tok >> 1) & 3)) << 4));
+                    uint4 u;
+                    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                                 : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "r"(from) : "memory");
+                    if (tok < rows) {
+                        uint16_t *dst = static_cast<uint16_t *>(p.out) + (mc + tok) * p.out_ld + nc;
+                        if (p.vec && nc + 7 < p.N) {
+                            *reinterpret_cast<uint4 *>(dst) = u;
+                        } else {
+                            const uint32_t w4[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                            for (int j = 0; j < 8; ++j)
+                                if (nc + j < p.N) dst[j] = (uint16_t)(w4[j >> 1] >> (16 * (j & 1)));
+                        }
+                    }
+                }
                 }
             }
             tc_fence_before();
@@ -320,7 +429,7 @@ __host__ __device__ constexpr uint32_t off_bar(int tn) { return STAGES * stage_b
 __host__ __device__ constexpr uint32_t smem_bytes(int tn) { return off_bar(tn) + NBAR * 8 + 32 + 1024; }
 static_assert(STAGES * W_BYTES >= 128u * 128u * 4u, "the sums fit in the stages' memory");
 
-template <int DT>
+template <int DT, bool GELU>
 __global__ void __launch_bounds__(THREADS)
 kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, const Params p, int S) {
     extern __shared__ uint8_t smem_raw[];
@@ -330,7 +439,7 @@ kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtenso
     auto bar = [&](int i) -> uint32_t { return bars + 8u * (uint32_t)i; };
     volatile uint32_t *misc = reinterpret_cast<volatile uint32_t *>(smem + off_bar(p.tn) + NBAR * 8);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + off_bar(p.tn) + NBAR * 8 + 4);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = tid >> 5;
     const int rank = (int)(blockIdx.x % (unsigned)S), tile = (int)(blockIdx.x / (unsigned)S);
     const int n0 = (tile % p.ncb) * 128;
     const int m0 = (tile / p.ncb) * p.tn;
@@ -442,29 +551,22 @@ kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtenso
         }
         const float xsv = p.xs[m];
         const int64_t at_out = m * p.out_ld + n0 + c;
-        float y[4];
+        float wsv[4], bv[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int n = n0 + c + j;
-            y[j] = n < p.N ? finish(a[j], __fmul_rn(xsv, p.ws[n]), p.bias ? load_any(p.bias, p.bias_dtype, n) : 0.f,
-                                    p.bias != nullptr, p.gelu != 0)
-                           : 0.f;
+            wsv[j] = n < p.N ? p.ws[n] : 0.f;
+            bv[j] = (p.bias && n < p.N) ? load_any(p.bias, p.bias_dtype, n) : 0.f;
         }
+        const uint64_t y01 = finish<GELU>(a[0], a[1], f2_mul(f2(xsv, xsv), f2(wsv[0], wsv[1])), f2(bv[0], bv[1]));
+        const uint64_t y23 = finish<GELU>(a[2], a[3], f2_mul(f2(xsv, xsv), f2(wsv[2], wsv[3])), f2(bv[2], bv[3]));
+        const float y[4] = {f2_lo(y01), f2_hi(y01), f2_lo(y23), f2_hi(y23)};
         if (p.vec && n0 + c + 3 < p.N) {
             if (DT == SS_F32) {
                 *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + at_out) = make_float4(y[0], y[1], y[2], y[3]);
             } else {
-                union {
-                    __nv_bfloat16 h[4];
-                    __half f[4];
-                    uint2 u;
-                } o;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if (DT == SS_F16) o.f[j] = __float2half_rn(y[j]);
-                    else o.h[j] = __float2bfloat16_rn(y[j]);
-                }
-                *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.out) + at_out) = o.u;
+                *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.out) + at_out) =
+                    make_uint2(pack2<DT>(y[0], y[1]), pack2<DT>(y[2], y[3]));
             }
         } else {
 #pragma unroll
@@ -493,12 +595,12 @@ static int g_lin_configured[SS_MAX_DEVICES];
 static void *g_lin_ctx[SS_MAX_DEVICES];
 static int g_lin_nsm[SS_MAX_DEVICES];
 
-template <int DT>
+template <int DT, bool GELU>
 static cudaError_t linear_i8_attributes() {
-    cudaError_t e = cudaFuncSetAttribute(lin::pair::kernel<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    cudaError_t e = cudaFuncSetAttribute(lin::pair::kernel<DT, GELU>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          (int)lin::pair::SMEM_BYTES);
     if (e != cudaSuccess) return e;
-    return cudaFuncSetAttribute(lin::split::kernel<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    return cudaFuncSetAttribute(lin::split::kernel<DT, GELU>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                 (int)lin::split::smem_bytes(lin::split::MAX_TN));
 }
 
@@ -509,9 +611,12 @@ int linear_i8_prepare(int device) {
     if (rc) return rc;
     std::lock_guard<std::mutex> lock(g_lin_mutex);
     if (g_lin_configured[device] && g_lin_ctx[device] == ctx) return 0;
-    cudaError_t e = linear_i8_attributes<SS_BF16>();
-    if (e == cudaSuccess) e = linear_i8_attributes<SS_F32>();
-    if (e == cudaSuccess) e = linear_i8_attributes<SS_F16>();
+    cudaError_t e = linear_i8_attributes<SS_BF16, false>();
+    if (e == cudaSuccess) e = linear_i8_attributes<SS_BF16, true>();
+    if (e == cudaSuccess) e = linear_i8_attributes<SS_F32, false>();
+    if (e == cudaSuccess) e = linear_i8_attributes<SS_F32, true>();
+    if (e == cudaSuccess) e = linear_i8_attributes<SS_F16, false>();
+    if (e == cudaSuccess) e = linear_i8_attributes<SS_F16, true>();
     int nsm = 0;
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&nsm, cudaDevAttrMultiProcessorCount, device);
     if (e != cudaSuccess) return (int)e;
@@ -549,7 +654,7 @@ static Plan choose(int M, int N, int K, int nsm) {
     return best;
 }
 
-template <int DT>
+template <int DT, bool GELU>
 static int launch(const Plan &plan, const int8_t *x, int64_t x_ld, const int8_t *w, int64_t w_ld, Params p, int nsm,
                   cudaStream_t st) {
     CUtensorMap tm_w, tm_x;
@@ -565,7 +670,7 @@ static int launch(const Plan &plan, const int8_t *x, int64_t x_ld, const int8_t 
         if (tiles > 0x7fffffff) return SS_ERR_SHAPE;
         p.ntiles = (int)tiles;
         const int npairs = (int)(tiles < nsm / 2 ? tiles : nsm / 2);
-        pair::kernel<DT><<<2 * npairs, pair::THREADS, pair::SMEM_BYTES, st>>>(tm_w, tm_x, p);
+        pair::kernel<DT, GELU><<<2 * npairs, pair::THREADS, pair::SMEM_BYTES, st>>>(tm_w, tm_x, p);
         return (int)cudaGetLastError();
     }
     p.ncb = (p.N + 127) / 128;
@@ -580,7 +685,7 @@ static int launch(const Plan &plan, const int8_t *x, int64_t x_ld, const int8_t 
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return (int)cudaLaunchKernelEx(&cfg, split::kernel<DT>, tm_w, tm_x, p, plan.S);
+    return (int)cudaLaunchKernelEx(&cfg, split::kernel<DT, GELU>, tm_w, tm_x, p, plan.S);
 }
 
 }  // namespace lin
@@ -605,12 +710,14 @@ extern "C" int ss_linear_i8(const int8_t *x, int64_t x_ld, const float *xs, cons
     if (rc) return rc;
     const int nsm = g_lin_nsm[device];
     lin::Params p = {};
-    p.xs = xs, p.ws = ws, p.bias = bias, p.bias_dtype = bias_dtype, p.gelu = gelu, p.out_dtype = out_dtype;
+    p.xs = xs, p.ws = ws, p.bias = bias, p.bias_dtype = bias_dtype;
     p.M = M, p.N = N, p.K = K, p.out = out, p.out_ld = out_ld, p.status = status;
-    p.vec = !lin::off(out, 4 * lin::type_bytes(out_dtype)) && out_ld % 4 == 0;
     const lin::Plan plan = lin::choose(M, N, K, nsm);
+    const size_t store = plan.pairs ? 16 : 4 * lin::type_bytes(out_dtype);   // bytes of a vector store
+    p.vec = !lin::off(out, store) && (size_t)out_ld * lin::type_bytes(out_dtype) % store == 0;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (out_dtype == SS_BF16) return lin::launch<SS_BF16>(plan, x, x_ld, w, w_ld, p, nsm, st);
-    if (out_dtype == SS_F16) return lin::launch<SS_F16>(plan, x, x_ld, w, w_ld, p, nsm, st);
-    return lin::launch<SS_F32>(plan, x, x_ld, w, w_ld, p, nsm, st);
+    auto go = [&](auto f) { return f(plan, x, x_ld, w, w_ld, p, nsm, st); };
+    if (out_dtype == SS_BF16) return go(gelu ? lin::launch<SS_BF16, true> : lin::launch<SS_BF16, false>);
+    if (out_dtype == SS_F16) return go(gelu ? lin::launch<SS_F16, true> : lin::launch<SS_F16, false>);
+    return go(gelu ? lin::launch<SS_F32, true> : lin::launch<SS_F32, false>);
 }
