@@ -42,6 +42,7 @@ struct Args {
     float *scales;
     int n, d, frame_tokens;
     float eps;
+    int out_words;          // the codes of a chunk leave as one aligned word
 };
 
 __device__ __forceinline__ float to_f(float v) { return v; }
@@ -64,8 +65,9 @@ __device__ __forceinline__ Scale row_scale(uint32_t m) {
     const float s = fmaxf(__fdiv_rn(__uint_as_float(m), 127.f), TINY);
     return {s, __frcp_rn(s)};
 }
-__device__ __forceinline__ int8_t code(float x, Scale s) {
-    return s.inv == 0.f ? (int8_t)0 : (int8_t)__float2int_rn(__fmul_rn(x, s.inv));
+// the code of x as the low byte: adding 1.5 * 2^23 rounds |x| < 2^22 to the nearest integer, ties to even
+__device__ __forceinline__ uint32_t code(float x, Scale s) {
+    return s.inv == 0.f ? 0u : __float_as_uint(__fadd_rn(__fmul_rn(x, s.inv), 12582912.f));
 }
 
 __device__ __forceinline__ float block_sum(float a, float *red) {
@@ -88,11 +90,182 @@ __device__ __forceinline__ uint32_t block_max(uint32_t a, uint32_t *red) {
     return m;
 }
 
-// One CTA per row, any width, stride and alignment: element loads, the row read once per statistic.
+template <int G>
+__device__ __forceinline__ float group_sum(float a, float *red) {
+    if constexpr (G > 32) {
+        return block_sum(a, red);
+    } else {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+        return a;
+    }
+}
+template <int G>
+__device__ __forceinline__ uint32_t group_max(uint32_t a, uint32_t *red) {
+    return G > 32 ? block_max(a, red) : __reduce_max_sync(0xffffffffu, a);
+}
+
+// values c .. c + VEC - 1 of a row of d, 0 past its end; AL: 16-byte loads (d a multiple of VEC)
+template <bool AL, typename T, int VEC>
+__device__ __forceinline__ void load_chunk(const T *src, int c, int d, float (&v)[VEC]) {
+    if constexpr (AL) {
+        union {
+            uint4 u[(VEC * sizeof(T) + 15) / 16];
+            T e[VEC];
+        } a;
+#pragma unroll
+        for (int i = 0; i < (int)(VEC * sizeof(T) / 16); ++i)
+            a.u[i] = c < d ? reinterpret_cast<const uint4 *>(src + c)[i] : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) v[j] = to_f(a.e[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) v[j] = c + j < d ? to_f(src[c + j]) : 0.f;
+    }
+}
+template <bool AL, typename T, int VEC>
+__device__ __forceinline__ void store_chunk(T *dst, int c, int d, const float (&v)[VEC]) {
+    if constexpr (AL) {
+        union {
+            uint4 u;
+            T e[VEC];
+        } a;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) from_f(v[j], a.e[j]);
+        if (c < d) *reinterpret_cast<uint4 *>(dst + c) = a.u;
+    } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+            if (c + j < d) from_f(v[j], dst[c + j]);
+    }
+}
+template <int VEC>
+__device__ __forceinline__ void store_codes(int8_t *out, int c, int d, int words, const float (&v)[VEC], Scale s) {
+    uint32_t k[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) k[j] = code(v[j], s);
+    if (words && c + VEC <= d) {
+        uint32_t o[VEC / 4];
+#pragma unroll
+        for (int j = 0; j < VEC / 4; ++j)
+            o[j] = __byte_perm(__byte_perm(k[4 * j], k[4 * j + 1], 0x0040),
+                               __byte_perm(k[4 * j + 2], k[4 * j + 3], 0x0040), 0x5410);
+        if constexpr (VEC == 8) *reinterpret_cast<uint2 *>(out + c) = make_uint2(o[0], o[1]);
+        else *reinterpret_cast<uint32_t *>(out + c) = o[0];
+    } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+            if (c + j < d) out[c + j] = (int8_t)k[j];
+    }
+}
+
+// One group of G threads per row, the row held in registers, NE values a thread: one read of each
+// input, one write of each output. Thread t takes chunks t, t + G, ... of VEC consecutive values:
+// 16-byte accesses where base and strides allow (AL; VEC = 8 or 4), else single values in chunks of
+// four, so that the codes still leave as whole words.
+template <typename T, int MODE, int G, int NE, bool AL>
+__global__ void __launch_bounds__(G < 128 ? 128 : G) row_kernel(const Args p) {
+    constexpr int VEC = AL ? 16 / (int)sizeof(T) : 4, NV = NE / VEC;
+    __shared__ float fred[G / 32];
+    __shared__ uint32_t ured[G / 32];
+    const int t = G == 32 ? (int)(threadIdx.x & 31) : (int)threadIdx.x, d = p.d;
+    const int64_t row = G == 32 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5) : (int64_t)blockIdx.x;
+    if (row >= p.n) return;   // whole warps (G = 32); no block barrier follows
+    const T *x = static_cast<const T *>(p.x) + row * p.x_ld;
+    const T *r = p.res ? static_cast<const T *>(p.res) + row * p.res_ld : nullptr;
+    T *sum = p.sum ? static_cast<T *>(p.sum) + row * p.sum_ld : nullptr;
+    const T *w = static_cast<const T *>(p.weight), *b = static_cast<const T *>(p.bias);
+    const int64_t f = (MODE == LN && p.frame_tokens > 0) ? row / p.frame_tokens : 0;
+    float v[NV][VEC];
+    float s = 0.f;
+    uint32_t m = 0u;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) load_chunk<AL>(x, (i * G + t) * VEC, d, v[i]);
+    if (MODE != QUANT && r) {
+        const float *g = p.gate ? p.gate + f * p.gate_ld : nullptr;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * G + t) * VEC;
+            float y[VEC];
+            load_chunk<AL>(r, c, d, y);
+            if (MODE == LN && g) {
+                float gv[VEC];
+                load_chunk<AL>(g, c, d, gv);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) y[j] = __fmul_rn(y[j], gv[j]);
+            }
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) v[i][j] = __fadd_rn(v[i][j], y[j]);
+            if (sum) store_chunk<AL>(sum, c, d, v[i]);   // this thread has read x and r here, no other does
+        }
+    }
+    float rstd = 1.f;
+    if (MODE == QUANT) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) m = max(m, abs_bits(v[i][j]));
+    } else if (MODE == RMS) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            float wv[VEC];
+            load_chunk<AL>(w, (i * G + t) * VEC, d, wv);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                s += v[i][j] * v[i][j];
+                v[i][j] = __fmul_rn(v[i][j], wv[j]);
+                m = max(m, abs_bits(v[i][j]));
+            }
+        }
+        rstd = rsqrtf(__fadd_rn(__fdiv_rn(group_sum<G>(s, fred), (float)d), p.eps));
+    } else {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) s += v[i][j];
+        const float mean = __fdiv_rn(group_sum<G>(s, fred), (float)d);
+        s = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j)
+                if ((i * G + t) * VEC + (AL ? 0 : j) < d) {
+                    v[i][j] -= mean;
+                    s += v[i][j] * v[i][j];
+                }
+        rstd = rsqrtf(__fadd_rn(__fdiv_rn(group_sum<G>(s, fred), (float)d), p.eps));
+        const float *sh = p.shift + f * p.mod_ld, *sc = p.scale + f * p.mod_ld;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * G + t) * VEC;
+            float a[VEC], e[VEC];
+            if (w) {
+                load_chunk<AL>(w, c, d, a);
+                load_chunk<AL>(b, c, d, e);
+            } else {
+                load_chunk<AL>(sc, c, d, a);
+                load_chunk<AL>(sh, c, d, e);
+            }
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                const float z = v[i][j] * rstd;
+                v[i][j] = w ? z * a[j] + e[j] : z * (1.f + a[j]) + e[j];
+                m = max(m, abs_bits(v[i][j]));
+            }
+        }
+    }
+    const Scale q = row_scale(group_max<G>(m, ured));
+    int8_t *out = p.out + row * p.out_ld;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) store_codes<VEC>(out, (i * G + t) * VEC, d, p.out_words, v[i], q);
+    if (t == 0) p.scales[row] = MODE == RMS ? __fmul_rn(q.s, rstd) : q.s;
+}
+
+// Rows too long for registers: one CTA per row, element loads, the row read once per statistic.
 template <typename T, int MODE>
-__global__ void __launch_bounds__(256) row_kernel(const Args p) {
-    __shared__ float fred[8];
-    __shared__ uint32_t ured[8];
+__global__ void __launch_bounds__(512) long_row_kernel(const Args p) {
+    __shared__ float fred[16];
+    __shared__ uint32_t ured[16];
     const int64_t row = blockIdx.x;
     const int t = threadIdx.x, d = p.d;
     const T *x = static_cast<const T *>(p.x) + row * p.x_ld;
@@ -136,7 +309,7 @@ __global__ void __launch_bounds__(256) row_kernel(const Args p) {
     const Scale s = row_scale(block_max(m, ured));
     for (int c = t; c < d; c += blockDim.x) {
         const float v = value(c);
-        p.out[row * p.out_ld + c] = code(coded(c, v), s);
+        p.out[row * p.out_ld + c] = (int8_t)code(coded(c, v), s);
         // after the last read of x[c] and r[c], by the thread that read them: the sum may be
         // written over either
         if (p.sum) from_f(v, static_cast<T *>(p.sum)[row * p.sum_ld + c]);
@@ -144,17 +317,41 @@ __global__ void __launch_bounds__(256) row_kernel(const Args p) {
     if (t == 0) p.scales[row] = MODE == RMS ? __fmul_rn(s.s, rstd) : s.s;
 }
 
-template <int MODE>
-static int launch(const Args &p, int dtype, cudaStream_t st) {
-    const unsigned threads = (unsigned)(p.d >= 256 ? 256 : (p.d + 31) / 32 * 32);
-    if (dtype == SS_BF16) row_kernel<__nv_bfloat16, MODE><<<p.n, threads, 0, st>>>(p);
-    else if (dtype == SS_F16) row_kernel<__half, MODE><<<p.n, threads, 0, st>>>(p);
-    else row_kernel<float, MODE><<<p.n, threads, 0, st>>>(p);
+static size_t type_bytes(int dtype) { return dtype == SS_F32 ? 4 : 2; }
+static bool off(const void *p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) != 0; }
+
+template <typename T, int MODE, bool AL>
+static int launch_rows(const Args &p, cudaStream_t st) {
+    const unsigned n = (unsigned)p.n;
+    if (p.d <= 32 * 48) row_kernel<T, MODE, 32, 48, AL><<<(n + 3) / 4, 128, 0, st>>>(p);
+    else if (p.d <= 128 * 16) row_kernel<T, MODE, 128, 16, AL><<<n, 128, 0, st>>>(p);
+    else if (p.d <= 128 * 40) row_kernel<T, MODE, 128, 40, AL><<<n, 128, 0, st>>>(p);
+    else if (p.d <= 256 * 40) row_kernel<T, MODE, 256, 40, AL><<<n, 256, 0, st>>>(p);
+    else if (p.d <= 512 * 48) row_kernel<T, MODE, 512, 48, AL><<<n, 512, 0, st>>>(p);
+    else long_row_kernel<T, MODE><<<n, 512, 0, st>>>(p);
     return (int)cudaGetLastError();
 }
 
-static size_t type_bytes(int dtype) { return dtype == SS_F32 ? 4 : 2; }
-static bool off(const void *p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) != 0; }
+template <typename T, int MODE>
+static int launch_type(Args p, cudaStream_t st) {
+    constexpr int VEC = 16 / (int)sizeof(T);
+    // rows and vectors all start at 16-byte boundaries and end at a whole vector
+    const bool al = p.d % VEC == 0 && !off(p.x, 16) && p.x_ld % VEC == 0 && !off(p.weight, 16) && !off(p.bias, 16) &&
+                    (!p.res || (!off(p.res, 16) && p.res_ld % VEC == 0)) &&
+                    (!p.sum || (!off(p.sum, 16) && p.sum_ld % VEC == 0)) &&
+                    (!p.gate || (!off(p.gate, 16) && p.gate_ld % 4 == 0)) &&
+                    (!p.shift || (!off(p.shift, 16) && !off(p.scale, 16) && p.mod_ld % 4 == 0));
+    const size_t word = al ? VEC : 4;
+    p.out_words = !off(p.out, word) && p.out_ld % (int64_t)word == 0;
+    return al ? launch_rows<T, MODE, true>(p, st) : launch_rows<T, MODE, false>(p, st);
+}
+
+template <int MODE>
+static int launch(const Args &p, int dtype, cudaStream_t st) {
+    if (dtype == SS_BF16) return launch_type<__nv_bfloat16, MODE>(p, st);
+    if (dtype == SS_F16) return launch_type<__half, MODE>(p, st);
+    return launch_type<float, MODE>(p, st);
+}
 
 // checks shared by the three entry points; 0 when the call is one the kernels can run
 static int check_rows(const Args &p, int dtype) {

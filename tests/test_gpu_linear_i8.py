@@ -46,7 +46,7 @@ def _check_codes(q, s, y, slack, s_tol):
     assert (q.abs().amax(1)[full] == 127).all()   # the largest value uses the whole range
 
 
-SIZES = [(1, 1), (1, 1536), (3, 5), (7, 8960), (33, 1537), (129, 256), (65, 2048), (4, 16391), (2, 40003), (1560, 1536)]
+SIZES = [(1, 1), (1, 1536), (3, 5), (7, 8960), (33, 1537), (129, 256), (65, 2048), (6, 5112), (5, 10240), (4, 16391), (3, 24576), (2, 40003), (1560, 1536)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
