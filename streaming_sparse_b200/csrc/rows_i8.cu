@@ -21,7 +21,7 @@ namespace rows {
 
 constexpr float TINY = 1e-30f;   // the smallest scale: a row of zeros keeps a finite reciprocal
 
-enum Mode { QUANT, RMS, LN };
+enum Mode { QUANT, RMS, MOD, AFFINE };   // MOD, AFFINE: the two forms of the LayerNorm
 
 struct Args {
     const void *x;
@@ -70,75 +70,86 @@ __device__ __forceinline__ uint32_t code(float x, Scale s) {
     return s.inv == 0.f ? 0u : __float_as_uint(__fadd_rn(__fmul_rn(x, s.inv), 12582912.f));
 }
 
-__device__ __forceinline__ float block_sum(float a, float *red) {
+// The block's reductions: warps by shuffles, then one word a warp through shared memory, with one
+// barrier each (consecutive reductions use the two halves of `red` in turn). Every thread adds the
+// warps' words in the same order.
+template <bool WARP>
+struct Reduce {
+    float2 (*red)[32];
+    int turn = 0;
+    __device__ __forceinline__ float2 operator()(float s, uint32_t m) {   // (sum of s, max of m's bits)
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = a;
-    __syncthreads();
-    float s = 0.f;
-    for (int i = 0; i < (int)(blockDim.x >> 5); ++i) s += red[i];   // the same order in every thread
-    return s;
-}
-__device__ __forceinline__ uint32_t block_max(uint32_t a, uint32_t *red) {
-    a = __reduce_max_sync(0xffffffffu, a);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = a;
-    __syncthreads();
-    uint32_t m = 0u;
-    for (int i = 0; i < (int)(blockDim.x >> 5); ++i) m = max(m, red[i]);
-    return m;
-}
+        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        m = __reduce_max_sync(0xffffffffu, m);
+        if (WARP || blockDim.x == 32) return make_float2(s, __uint_as_float(m));
+        const int nw = blockDim.x >> 5, lane = threadIdx.x & 31;
+        if (lane == 0) red[turn][threadIdx.x >> 5] = make_float2(s, __uint_as_float(m));
+        __syncthreads();
+        if (nw <= 8) {
+            float2 a = red[turn][0];
+            uint32_t top = __float_as_uint(a.y);
+            for (int i = 1; i < nw; ++i) {
+                const float2 b = red[turn][i];
+                a.x += b.x;
+                top = max(top, __float_as_uint(b.y));
+            }
+            a.y = __uint_as_float(top);
+            turn ^= 1;
+            return a;
+        }
+        const float2 a = lane < nw ? red[turn][lane] : make_float2(0.f, 0.f);
+        s = a.x;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        turn ^= 1;
+        return make_float2(s, __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(a.y))));
+    }
+    __device__ __forceinline__ float sum(float s) { return (*this)(s, 0u).x; }
+    __device__ __forceinline__ uint32_t max_bits(uint32_t m) { return __float_as_uint((*this)(0.f, m).y); }
+};
 
-template <int G>
-__device__ __forceinline__ float group_sum(float a, float *red) {
-    if constexpr (G > 32) {
-        return block_sum(a, red);
-    } else {
+// VEC values of a row of d from c on, as loaded: 16 bytes at once (AL, d a multiple of VEC), or one by
+// one; zeros past the row's end
+template <typename T, int VEC, bool AL>
+struct Chunk {
+    static constexpr int WORDS = (VEC * (int)sizeof(T) + 15) / 16;
+    union {
+        uint4 u[WORDS];
+        T e[VEC];
+    };
+    __device__ __forceinline__ Chunk() {
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
-        return a;
+        for (int i = 0; i < WORDS; ++i) u[i] = make_uint4(0u, 0u, 0u, 0u);
     }
-}
-template <int G>
-__device__ __forceinline__ uint32_t group_max(uint32_t a, uint32_t *red) {
-    return G > 32 ? block_max(a, red) : __reduce_max_sync(0xffffffffu, a);
-}
+    __device__ __forceinline__ void load(const T *src, int c, int d) {
+        if constexpr (AL) {
+#pragma unroll
+            for (int i = 0; i < WORDS; ++i)
+                u[i] = c < d ? reinterpret_cast<const uint4 *>(src + c)[i] : make_uint4(0u, 0u, 0u, 0u);
+        } else {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                T z;
+                from_f(0.f, z);
+                e[j] = c + j < d ? src[c + j] : z;
+            }
+        }
+    }
+    __device__ __forceinline__ void store(T *dst, int c, int d) const {
+        if constexpr (AL) {
+#pragma unroll
+            for (int i = 0; i < WORDS; ++i)
+                if (c < d) reinterpret_cast<uint4 *>(dst + c)[i] = u[i];
+        } else {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j)
+                if (c + j < d) dst[c + j] = e[j];
+        }
+    }
+    __device__ __forceinline__ float operator[](int j) const { return to_f(e[j]); }
+    __device__ __forceinline__ void set(int j, float v) { from_f(v, e[j]); }
+};
 
-// values c .. c + VEC - 1 of a row of d, 0 past its end; AL: 16-byte loads (d a multiple of VEC)
-template <bool AL, typename T, int VEC>
-__device__ __forceinline__ void load_chunk(const T *src, int c, int d, float (&v)[VEC]) {
-    if constexpr (AL) {
-        union {
-            uint4 u[(VEC * sizeof(T) + 15) / 16];
-            T e[VEC];
-        } a;
-#pragma unroll
-        for (int i = 0; i < (int)(VEC * sizeof(T) / 16); ++i)
-            a.u[i] = c < d ? reinterpret_cast<const uint4 *>(src + c)[i] : make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) v[j] = to_f(a.e[j]);
-    } else {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) v[j] = c + j < d ? to_f(src[c + j]) : 0.f;
-    }
-}
-template <bool AL, typename T, int VEC>
-__device__ __forceinline__ void store_chunk(T *dst, int c, int d, const float (&v)[VEC]) {
-    if constexpr (AL) {
-        union {
-            uint4 u;
-            T e[VEC];
-        } a;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) from_f(v[j], a.e[j]);
-        if (c < d) *reinterpret_cast<uint4 *>(dst + c) = a.u;
-    } else {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j)
-            if (c + j < d) from_f(v[j], dst[c + j]);
-    }
-}
 template <int VEC>
 __device__ __forceinline__ void store_codes(int8_t *out, int c, int d, int words, const float (&v)[VEC], Scale s) {
     uint32_t k[VEC];
@@ -159,118 +170,139 @@ __device__ __forceinline__ void store_codes(int8_t *out, int c, int d, int words
     }
 }
 
-// One group of G threads per row, the row held in registers, NE values a thread: one read of each
-// input, one write of each output. Thread t takes chunks t, t + G, ... of VEC consecutive values:
-// 16-byte accesses where base and strides allow (AL; VEC = 8 or 4), else single values in chunks of
-// four, so that the codes still leave as whole words.
-template <typename T, int MODE, int G, int NE, bool AL>
-__global__ void __launch_bounds__(G < 128 ? 128 : G) row_kernel(const Args p) {
+// The row in registers, NE values a thread: one read of each input, one write of each output. WARP: a
+// warp per row (four rows a block), reductions by shuffles alone; else a block per row, as many threads
+// as its chunks need. Thread t takes chunks t, t + threads, ... of VEC consecutive values: 16-byte
+// accesses where base and strides allow (AL; VEC = 8 or 4), else single values in chunks of four, so
+// that the codes still leave as whole words. All of x and the residual is asked for before the first
+// value is used or the sum is stored: the sum may lie over either, so no load may pass a store.
+template <typename T, int MODE, bool WARP, int NE, bool AL>
+__global__ void __launch_bounds__(WARP ? 128 : NE == 16 ? 128 : NE == 40 ? 256 : 512) row_kernel(const Args p) {
     constexpr int VEC = AL ? 16 / (int)sizeof(T) : 4, NV = NE / VEC;
-    __shared__ float fred[G / 32];
-    __shared__ uint32_t ured[G / 32];
-    const int t = G == 32 ? (int)(threadIdx.x & 31) : (int)threadIdx.x, d = p.d;
-    const int64_t row = G == 32 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5) : (int64_t)blockIdx.x;
-    if (row >= p.n) return;   // whole warps (G = 32); no block barrier follows
-    const T *x = static_cast<const T *>(p.x) + row * p.x_ld;
-    const T *r = p.res ? static_cast<const T *>(p.res) + row * p.res_ld : nullptr;
-    T *sum = p.sum ? static_cast<T *>(p.sum) + row * p.sum_ld : nullptr;
+    __shared__ float2 red[2][32];
+    Reduce<WARP> reduce{red};
+    const int t = WARP ? (int)(threadIdx.x & 31) : (int)threadIdx.x, G = WARP ? 32 : (int)blockDim.x, d = p.d;
+    const int64_t row = WARP ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5) : (int64_t)blockIdx.x;
+    if (row >= p.n) return;   // whole warps (WARP); no block barrier follows
+    const T *x = static_cast<const T *>(p.x) + row * p.x_ld, *r = static_cast<const T *>(p.res) + row * p.res_ld;
     const T *w = static_cast<const T *>(p.weight), *b = static_cast<const T *>(p.bias);
-    const int64_t f = (MODE == LN && p.frame_tokens > 0) ? row / p.frame_tokens : 0;
+    const int64_t f = (MODE >= MOD && p.frame_tokens > 0) ? row / p.frame_tokens : 0;
+    auto at = [&](int i) { return (i * G + t) * VEC; };
     float v[NV][VEC];
-    float s = 0.f;
-    uint32_t m = 0u;
+    {
+        Chunk<T, VEC, AL> xv[NV], rv[NV];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) load_chunk<AL>(x, (i * G + t) * VEC, d, v[i]);
-    if (MODE != QUANT && r) {
-        const float *g = p.gate ? p.gate + f * p.gate_ld : nullptr;
+        for (int i = 0; i < NV; ++i) xv[i].load(x, at(i), d);
+        if (MODE != QUANT && p.res) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = (i * G + t) * VEC;
-            float y[VEC];
-            load_chunk<AL>(r, c, d, y);
-            if (MODE == LN && g) {
-                float gv[VEC];
-                load_chunk<AL>(g, c, d, gv);
+            for (int i = 0; i < NV; ++i) rv[i].load(r, at(i), d);
+        }
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) y[j] = __fmul_rn(y[j], gv[j]);
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) v[i][j] = xv[i][j];
+        if (MODE != QUANT && p.res) {
+            if (MODE >= MOD && p.gate) {
+#pragma unroll
+                for (int i = 0; i < NV; ++i) {
+                    Chunk<float, VEC, AL> g;
+                    g.load(p.gate + f * p.gate_ld, at(i), d);
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) v[i][j] = __fadd_rn(v[i][j], __fmul_rn(rv[i][j], g[j]));
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < NV; ++i)
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) v[i][j] = __fadd_rn(v[i][j], rv[i][j]);
             }
+            if (p.sum) {
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) v[i][j] = __fadd_rn(v[i][j], y[j]);
-            if (sum) store_chunk<AL>(sum, c, d, v[i]);   // this thread has read x and r here, no other does
+                for (int i = 0; i < NV; ++i) {
+                    Chunk<T, VEC, AL> o;
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) o.set(j, v[i][j]);
+                    o.store(static_cast<T *>(p.sum) + row * p.sum_ld, at(i), d);
+                }
+            }
         }
     }
-    float rstd = 1.f;
+    float s = 0.f, rstd = 1.f;
+    uint32_t m = 0u;
     if (MODE == QUANT) {
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int j = 0; j < VEC; ++j) m = max(m, abs_bits(v[i][j]));
+        m = reduce.max_bits(m);
     } else if (MODE == RMS) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            float wv[VEC];
-            load_chunk<AL>(w, (i * G + t) * VEC, d, wv);
+            Chunk<T, VEC, AL> a;
+            a.load(w, at(i), d);
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
                 s += v[i][j] * v[i][j];
-                v[i][j] = __fmul_rn(v[i][j], wv[j]);
+                v[i][j] = __fmul_rn(v[i][j], a[j]);
                 m = max(m, abs_bits(v[i][j]));
             }
         }
-        rstd = rsqrtf(__fadd_rn(__fdiv_rn(group_sum<G>(s, fred), (float)d), p.eps));
+        const float2 a = reduce(s, m);
+        rstd = rsqrtf(__fadd_rn(__fdiv_rn(a.x, (float)d), p.eps));
+        m = __float_as_uint(a.y);
     } else {
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int j = 0; j < VEC; ++j) s += v[i][j];
-        const float mean = __fdiv_rn(group_sum<G>(s, fred), (float)d);
+        const float mean = __fdiv_rn(reduce.sum(s), (float)d);
         s = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int j = 0; j < VEC; ++j)
-                if ((i * G + t) * VEC + (AL ? 0 : j) < d) {
+                if (at(i) + (AL ? 0 : j) < d) {
                     v[i][j] -= mean;
                     s += v[i][j] * v[i][j];
                 }
-        rstd = rsqrtf(__fadd_rn(__fdiv_rn(group_sum<G>(s, fred), (float)d), p.eps));
-        const float *sh = p.shift + f * p.mod_ld, *sc = p.scale + f * p.mod_ld;
+        rstd = rsqrtf(__fadd_rn(__fdiv_rn(reduce.sum(s), (float)d), p.eps));
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = (i * G + t) * VEC;
-            float a[VEC], e[VEC];
-            if (w) {
-                load_chunk<AL>(w, c, d, a);
-                load_chunk<AL>(b, c, d, e);
+            if (MODE == AFFINE) {
+                Chunk<T, VEC, AL> a, e;
+                a.load(w, at(i), d);
+                e.load(b, at(i), d);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) v[i][j] = v[i][j] * rstd * a[j] + e[j];
             } else {
-                load_chunk<AL>(sc, c, d, a);
-                load_chunk<AL>(sh, c, d, e);
+                Chunk<float, VEC, AL> a, e;
+                a.load(p.scale + f * p.mod_ld, at(i), d);
+                e.load(p.shift + f * p.mod_ld, at(i), d);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) v[i][j] = v[i][j] * rstd * (1.f + a[j]) + e[j];
             }
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                const float z = v[i][j] * rstd;
-                v[i][j] = w ? z * a[j] + e[j] : z * (1.f + a[j]) + e[j];
-                m = max(m, abs_bits(v[i][j]));
-            }
+            for (int j = 0; j < VEC; ++j) m = max(m, abs_bits(v[i][j]));
         }
+        m = reduce.max_bits(m);
     }
-    const Scale q = row_scale(group_max<G>(m, ured));
+    const Scale q = row_scale(m);
     int8_t *out = p.out + row * p.out_ld;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) store_codes<VEC>(out, (i * G + t) * VEC, d, p.out_words, v[i], q);
+    for (int i = 0; i < NV; ++i) store_codes<VEC>(out, at(i), d, p.out_words, v[i], q);
     if (t == 0) p.scales[row] = MODE == RMS ? __fmul_rn(q.s, rstd) : q.s;
 }
 
 // Rows too long for registers: one CTA per row, element loads, the row read once per statistic.
 template <typename T, int MODE>
 __global__ void __launch_bounds__(512) long_row_kernel(const Args p) {
-    __shared__ float fred[16];
-    __shared__ uint32_t ured[16];
+    __shared__ float2 red[2][32];
+    Reduce<false> reduce{red};
     const int64_t row = blockIdx.x;
     const int t = threadIdx.x, d = p.d;
     const T *x = static_cast<const T *>(p.x) + row * p.x_ld;
     const T *r = p.res ? static_cast<const T *>(p.res) + row * p.res_ld : nullptr;
-    const int64_t f = (MODE == LN && p.frame_tokens > 0) ? row / p.frame_tokens : 0;
+    const int64_t f = (MODE >= MOD && p.frame_tokens > 0) ? row / p.frame_tokens : 0;
     const float *g = p.gate ? p.gate + f * p.gate_ld : nullptr;
     const T *w = static_cast<const T *>(p.weight), *b = static_cast<const T *>(p.bias);
     const float *sh = p.shift + f * p.mod_ld, *sc = p.scale + f * p.mod_ld;
@@ -286,27 +318,27 @@ __global__ void __launch_bounds__(512) long_row_kernel(const Args p) {
             const float v = value(c);
             s += v * v;
         }
-        rstd = rsqrtf(__fadd_rn(__fdiv_rn(block_sum(s, fred), (float)d), p.eps));
-    } else if (MODE == LN) {
+        rstd = rsqrtf(__fadd_rn(__fdiv_rn(reduce.sum(s), (float)d), p.eps));
+    } else if (MODE >= MOD) {
         float s = 0.f;
         for (int c = t; c < d; c += blockDim.x) s += value(c);
-        mean = __fdiv_rn(block_sum(s, fred), (float)d);
+        mean = __fdiv_rn(reduce.sum(s), (float)d);
         s = 0.f;
         for (int c = t; c < d; c += blockDim.x) {
             const float z = value(c) - mean;
             s += z * z;
         }
-        rstd = rsqrtf(__fadd_rn(__fdiv_rn(block_sum(s, fred), (float)d), p.eps));
+        rstd = rsqrtf(__fadd_rn(__fdiv_rn(reduce.sum(s), (float)d), p.eps));
     }
     auto coded = [&](int c, float v) -> float {   // what the codes stand for, up to RMS's rsqrt
         if (MODE == QUANT) return v;
         if (MODE == RMS) return __fmul_rn(v, to_f(w[c]));
         const float z = (v - mean) * rstd;
-        return w ? z * to_f(w[c]) + to_f(b[c]) : z * (1.f + sc[c]) + sh[c];
+        return MODE == AFFINE ? z * to_f(w[c]) + to_f(b[c]) : z * (1.f + sc[c]) + sh[c];
     };
     uint32_t m = 0u;
     for (int c = t; c < d; c += blockDim.x) m = max(m, abs_bits(coded(c, value(c))));
-    const Scale s = row_scale(block_max(m, ured));
+    const Scale s = row_scale(reduce.max_bits(m));
     for (int c = t; c < d; c += blockDim.x) {
         const float v = value(c);
         p.out[row * p.out_ld + c] = (int8_t)code(coded(c, v), s);
@@ -320,15 +352,19 @@ __global__ void __launch_bounds__(512) long_row_kernel(const Args p) {
 static size_t type_bytes(int dtype) { return dtype == SS_F32 ? 4 : 2; }
 static bool off(const void *p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) != 0; }
 
+template <typename T, int MODE, int NE, bool AL>
+static void launch_blocks(const Args &p, cudaStream_t st) {
+    constexpr int VEC = AL ? 16 / (int)sizeof(T) : 4, NV = NE / VEC;
+    const int chunks = (p.d + VEC - 1) / VEC;
+    row_kernel<T, MODE, false, NE, AL><<<p.n, ((chunks + NV - 1) / NV + 31) / 32 * 32, 0, st>>>(p);
+}
 template <typename T, int MODE, bool AL>
 static int launch_rows(const Args &p, cudaStream_t st) {
-    const unsigned n = (unsigned)p.n;
-    if (p.d <= 32 * 48) row_kernel<T, MODE, 32, 48, AL><<<(n + 3) / 4, 128, 0, st>>>(p);
-    else if (p.d <= 128 * 16) row_kernel<T, MODE, 128, 16, AL><<<n, 128, 0, st>>>(p);
-    else if (p.d <= 128 * 40) row_kernel<T, MODE, 128, 40, AL><<<n, 128, 0, st>>>(p);
-    else if (p.d <= 256 * 40) row_kernel<T, MODE, 256, 40, AL><<<n, 256, 0, st>>>(p);
-    else if (p.d <= 512 * 48) row_kernel<T, MODE, 512, 48, AL><<<n, 512, 0, st>>>(p);
-    else long_row_kernel<T, MODE><<<n, 512, 0, st>>>(p);
+    if (p.d <= 32 * 48) row_kernel<T, MODE, true, 48, AL><<<(unsigned)(((int64_t)p.n + 3) / 4), 128, 0, st>>>(p);
+    else if (p.d <= 128 * 16) launch_blocks<T, MODE, 16, AL>(p, st);
+    else if (p.d <= 256 * 40) launch_blocks<T, MODE, 40, AL>(p, st);
+    else if (p.d <= 512 * 48) launch_blocks<T, MODE, 48, AL>(p, st);
+    else long_row_kernel<T, MODE><<<p.n, 512, 0, st>>>(p);
     return (int)cudaGetLastError();
 }
 
@@ -410,5 +446,6 @@ extern "C" int ss_adaln_i8(const void *x, int64_t x_ld, const void *y, int64_t y
         return SS_ERR_SHAPE;
     const int rc = check_rows(p, dtype);
     if (rc || n == 0) return rc;
-    return launch<LN>(p, dtype, static_cast<cudaStream_t>(stream));
+    return affine ? launch<AFFINE>(p, dtype, static_cast<cudaStream_t>(stream))
+                  : launch<MOD>(p, dtype, static_cast<cudaStream_t>(stream));
 }
