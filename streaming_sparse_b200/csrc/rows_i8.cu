@@ -52,22 +52,34 @@ __device__ __forceinline__ void from_f(float v, float &o) { o = v; }
 __device__ __forceinline__ void from_f(float v, __nv_bfloat16 &o) { o = __float2bfloat16_rn(v); }
 __device__ __forceinline__ void from_f(float v, __half &o) { o = __float2half_rn(v); }
 
-// |x| as an unsigned integer orders the finite numbers, then infinity, then the NaNs: one integer
-// maximum finds the largest magnitude and keeps what is not finite.
-__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+// Magnitudes are compared as floats that keep a NaN, and between threads by their bits, whose order as
+// unsigned integers is the finite numbers, infinity, the NaNs.
+// the larger magnitude; a NaN stays one
+__device__ __forceinline__ float max_abs(float m, float x) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(m), "f"(fabsf(x)));
+    return r;
+}
+
+// two sums that no product before them is fused into
+__device__ __forceinline__ uint64_t add_both(uint64_t a, uint64_t b) {
+    return f2(__fadd_rn(f2_lo(a), f2_lo(b)), __fadd_rn(f2_hi(a), f2_hi(b)));
+}
 
 struct Scale {
     float s, inv;
+    uint32_t keep;   // all ones; 0 in a row whose codes are 0
 };
 // the scale of a row from the largest magnitude's bits; codes rint(x * inv) are within +-127
 __device__ __forceinline__ Scale row_scale(uint32_t m) {
-    if (m >= 0x7f800000u) return {__uint_as_float(0x7fc00000u), 0.f};
+    if (m >= 0x7f800000u) return {__uint_as_float(0x7fc00000u), 0.f, 0u};
     const float s = fmaxf(__fdiv_rn(__uint_as_float(m), 127.f), TINY);
-    return {s, __frcp_rn(s)};
+    return {s, __frcp_rn(s), ~0u};
 }
-// the code of x as the low byte: adding 1.5 * 2^23 rounds |x| < 2^22 to the nearest integer, ties to even
+// the code of x is the low byte: adding 1.5 * 2^23 rounds |x| < 2^22 to the nearest integer, ties to even
+constexpr float ROUND = 12582912.f;
 __device__ __forceinline__ uint32_t code(float x, Scale s) {
-    return s.inv == 0.f ? 0u : __float_as_uint(__fadd_rn(__fmul_rn(x, s.inv), 12582912.f));
+    return __float_as_uint(__fadd_rn(__fmul_rn(x, s.inv), ROUND)) & s.keep;
 }
 
 // The block's reductions: warps by shuffles, then one word a warp through shared memory, with one
@@ -146,27 +158,35 @@ struct Chunk {
                 if (c + j < d) dst[c + j] = e[j];
         }
     }
-    __device__ __forceinline__ float operator[](int j) const { return to_f(e[j]); }
-    __device__ __forceinline__ void set(int j, float v) { from_f(v, e[j]); }
+    // values 2 j and 2 j + 1
+    __device__ __forceinline__ uint64_t operator[](int j) const { return f2(to_f(e[2 * j]), to_f(e[2 * j + 1])); }
+    __device__ __forceinline__ void set(int j, uint64_t v) {
+        from_f(f2_lo(v), e[2 * j]);
+        from_f(f2_hi(v), e[2 * j + 1]);
+    }
 };
 
 template <int VEC>
-__device__ __forceinline__ void store_codes(int8_t *out, int c, int d, int words, const float (&v)[VEC], Scale s) {
+__device__ __forceinline__ void store_codes(int8_t *out, int c, int d, int words, const uint64_t (&v)[VEC / 2], Scale s) {
     uint32_t k[VEC];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) k[j] = code(v[j], s);
-    if (words && c + VEC <= d) {
-        uint32_t o[VEC / 4];
+    for (int j = 0; j < VEC / 2; ++j) {
+        const uint64_t y = f2_mul(v[j], f2(s.inv, s.inv));
+        k[2 * j] = __float_as_uint(__fadd_rn(f2_lo(y), ROUND));
+        k[2 * j + 1] = __float_as_uint(__fadd_rn(f2_hi(y), ROUND));
+    }
+    uint32_t o[VEC / 4];
 #pragma unroll
-        for (int j = 0; j < VEC / 4; ++j)
-            o[j] = __byte_perm(__byte_perm(k[4 * j], k[4 * j + 1], 0x0040),
-                               __byte_perm(k[4 * j + 2], k[4 * j + 3], 0x0040), 0x5410);
+    for (int j = 0; j < VEC / 4; ++j)
+        o[j] = s.keep & __byte_perm(__byte_perm(k[4 * j], k[4 * j + 1], 0x0040),
+                                    __byte_perm(k[4 * j + 2], k[4 * j + 3], 0x0040), 0x5410);
+    if (words && c + VEC <= d) {
         if constexpr (VEC == 8) *reinterpret_cast<uint2 *>(out + c) = make_uint2(o[0], o[1]);
         else *reinterpret_cast<uint32_t *>(out + c) = o[0];
     } else {
 #pragma unroll
         for (int j = 0; j < VEC; ++j)
-            if (c + j < d) out[c + j] = (int8_t)k[j];
+            if (c + j < d) out[c + j] = (int8_t)(o[j / 4] >> (8 * (j % 4)));
     }
 }
 
@@ -177,7 +197,8 @@ __device__ __forceinline__ void store_codes(int8_t *out, int c, int d, int words
 // that the codes still leave as whole words. All of x and the residual is asked for before the first
 // value is used or the sum is stored: the sum may lie over either, so no load may pass a store.
 template <typename T, int MODE, bool WARP, int NE, bool AL>
-__global__ void __launch_bounds__(WARP ? 128 : NE == 16 ? 128 : NE == 40 ? 256 : 512) row_kernel(const Args p) {
+__global__ void __launch_bounds__(WARP ? 128 : NE == 16 ? 128 : NE == 24 ? 1024 : NE == 40 ? 256 : 512,
+                                  NE == 48 && MODE == QUANT && !WARP ? 2 : 0) row_kernel(const Args p) {
     constexpr int VEC = AL ? 16 / (int)sizeof(T) : 4, NV = NE / VEC;
     __shared__ float2 red[2][32];
     Reduce<WARP> reduce{red};
@@ -186,9 +207,9 @@ __global__ void __launch_bounds__(WARP ? 128 : NE == 16 ? 128 : NE == 40 ? 256 :
     if (row >= p.n) return;   // whole warps (WARP); no block barrier follows
     const T *x = static_cast<const T *>(p.x) + row * p.x_ld, *r = static_cast<const T *>(p.res) + row * p.res_ld;
     const T *w = static_cast<const T *>(p.weight), *b = static_cast<const T *>(p.bias);
-    const int64_t f = (MODE >= MOD && p.frame_tokens > 0) ? row / p.frame_tokens : 0;
+    const int64_t f = (MODE >= MOD && p.frame_tokens > 0) ? (unsigned)row / (unsigned)p.frame_tokens : 0;
     auto at = [&](int i) { return (i * G + t) * VEC; };
-    float v[NV][VEC];
+    uint64_t v[NV][VEC / 2];   // pairs of values
     {
         Chunk<T, VEC, AL> xv[NV], rv[NV];
 #pragma unroll
@@ -200,7 +221,7 @@ __global__ void __launch_bounds__(WARP ? 128 : NE == 16 ? 128 : NE == 40 ? 256 :
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) v[i][j] = xv[i][j];
+            for (int j = 0; j < VEC / 2; ++j) v[i][j] = xv[i][j];
         if (MODE != QUANT && p.res) {
             if (MODE >= MOD && p.gate) {
 #pragma unroll
@@ -208,64 +229,70 @@ __global__ void __launch_bounds__(WARP ? 128 : NE == 16 ? 128 : NE == 40 ? 256 :
                     Chunk<float, VEC, AL> g;
                     g.load(p.gate + f * p.gate_ld, at(i), d);
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) v[i][j] = __fadd_rn(v[i][j], __fmul_rn(rv[i][j], g[j]));
+                    for (int j = 0; j < VEC / 2; ++j) v[i][j] = add_both(v[i][j], f2_mul(rv[i][j], g[j]));
                 }
             } else {
 #pragma unroll
                 for (int i = 0; i < NV; ++i)
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) v[i][j] = __fadd_rn(v[i][j], rv[i][j]);
+                    for (int j = 0; j < VEC / 2; ++j) v[i][j] = f2_add(v[i][j], rv[i][j]);
             }
             if (p.sum) {
 #pragma unroll
                 for (int i = 0; i < NV; ++i) {
                     Chunk<T, VEC, AL> o;
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) o.set(j, v[i][j]);
+                    for (int j = 0; j < VEC / 2; ++j) o.set(j, v[i][j]);
                     o.store(static_cast<T *>(p.sum) + row * p.sum_ld, at(i), d);
                 }
             }
         }
     }
-    float s = 0.f, rstd = 1.f;
-    uint32_t m = 0u;
+    float rstd = 1.f, m = 0.f;
+    uint64_t s2 = 0ull;
+    uint32_t top;
     if (MODE == QUANT) {
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) m = max(m, abs_bits(v[i][j]));
-        m = reduce.max_bits(m);
+            for (int j = 0; j < VEC / 2; ++j) m = max_abs(max_abs(m, f2_lo(v[i][j])), f2_hi(v[i][j]));
+        top = reduce.max_bits(__float_as_uint(m));
     } else if (MODE == RMS) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             Chunk<T, VEC, AL> a;
             a.load(w, at(i), d);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                s += v[i][j] * v[i][j];
-                v[i][j] = __fmul_rn(v[i][j], a[j]);
-                m = max(m, abs_bits(v[i][j]));
+            for (int j = 0; j < VEC / 2; ++j) {
+                s2 = f2_fma(v[i][j], v[i][j], s2);
+                v[i][j] = f2_mul(v[i][j], a[j]);
+                m = max_abs(max_abs(m, f2_lo(v[i][j])), f2_hi(v[i][j]));
             }
         }
-        const float2 a = reduce(s, m);
+        const float2 a = reduce(f2_lo(s2) + f2_hi(s2), __float_as_uint(m));
         rstd = rsqrtf(__fadd_rn(__fdiv_rn(a.x, (float)d), p.eps));
-        m = __float_as_uint(a.y);
+        top = __float_as_uint(a.y);
     } else {
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) s += v[i][j];
-        const float mean = __fdiv_rn(reduce.sum(s), (float)d);
-        s = 0.f;
+            for (int j = 0; j < VEC / 2; ++j) s2 = f2_add(s2, v[i][j]);
+        const float mean = __fdiv_rn(reduce.sum(f2_lo(s2) + f2_hi(s2)), (float)d);
+        s2 = 0ull;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
-            for (int j = 0; j < VEC; ++j)
-                if (at(i) + (AL ? 0 : j) < d) {
-                    v[i][j] -= mean;
-                    s += v[i][j] * v[i][j];
+            for (int j = 0; j < VEC / 2; ++j) {
+                if constexpr (AL) {   // past the row's end v stays 0
+                    if (at(i) < d) v[i][j] = f2_add(v[i][j], f2(-mean, -mean));
+                } else {
+                    const uint64_t z = f2_add(v[i][j], f2(-mean, -mean));
+                    v[i][j] = f2(at(i) + 2 * j < d ? f2_lo(z) : 0.f, at(i) + 2 * j + 1 < d ? f2_hi(z) : 0.f);
                 }
-        rstd = rsqrtf(__fadd_rn(__fdiv_rn(reduce.sum(s), (float)d), p.eps));
+                s2 = f2_fma(v[i][j], v[i][j], s2);
+            }
+        rstd = rsqrtf(__fadd_rn(__fdiv_rn(reduce.sum(f2_lo(s2) + f2_hi(s2)), (float)d), p.eps));
+        const uint64_t rstd2 = f2(rstd, rstd);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             if (MODE == AFFINE) {
@@ -273,20 +300,20 @@ __global__ void __launch_bounds__(WARP ? 128 : NE == 16 ? 128 : NE == 40 ? 256 :
                 a.load(w, at(i), d);
                 e.load(b, at(i), d);
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) v[i][j] = v[i][j] * rstd * a[j] + e[j];
+                for (int j = 0; j < VEC / 2; ++j) v[i][j] = f2_fma(v[i][j], f2_mul(rstd2, a[j]), e[j]);
             } else {
                 Chunk<float, VEC, AL> a, e;
                 a.load(p.scale + f * p.mod_ld, at(i), d);
                 e.load(p.shift + f * p.mod_ld, at(i), d);
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) v[i][j] = v[i][j] * rstd * (1.f + a[j]) + e[j];
+                for (int j = 0; j < VEC / 2; ++j) v[i][j] = f2_fma(v[i][j], f2_fma(rstd2, a[j], rstd2), e[j]);
             }
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) m = max(m, abs_bits(v[i][j]));
+            for (int j = 0; j < VEC / 2; ++j) m = max_abs(max_abs(m, f2_lo(v[i][j])), f2_hi(v[i][j]));
         }
-        m = reduce.max_bits(m);
+        top = reduce.max_bits(__float_as_uint(m));
     }
-    const Scale q = row_scale(m);
+    const Scale q = row_scale(top);
     int8_t *out = p.out + row * p.out_ld;
 #pragma unroll
     for (int i = 0; i < NV; ++i) store_codes<VEC>(out, at(i), d, p.out_words, v[i], q);
@@ -302,7 +329,7 @@ __global__ void __launch_bounds__(512) long_row_kernel(const Args p) {
     const int t = threadIdx.x, d = p.d;
     const T *x = static_cast<const T *>(p.x) + row * p.x_ld;
     const T *r = p.res ? static_cast<const T *>(p.res) + row * p.res_ld : nullptr;
-    const int64_t f = (MODE >= MOD && p.frame_tokens > 0) ? row / p.frame_tokens : 0;
+    const int64_t f = (MODE >= MOD && p.frame_tokens > 0) ? (unsigned)row / (unsigned)p.frame_tokens : 0;
     const float *g = p.gate ? p.gate + f * p.gate_ld : nullptr;
     const T *w = static_cast<const T *>(p.weight), *b = static_cast<const T *>(p.bias);
     const float *sh = p.shift + f * p.mod_ld, *sc = p.scale + f * p.mod_ld;
@@ -336,9 +363,9 @@ __global__ void __launch_bounds__(512) long_row_kernel(const Args p) {
         const float z = (v - mean) * rstd;
         return MODE == AFFINE ? z * to_f(w[c]) + to_f(b[c]) : z * (1.f + sc[c]) + sh[c];
     };
-    uint32_t m = 0u;
-    for (int c = t; c < d; c += blockDim.x) m = max(m, abs_bits(coded(c, value(c))));
-    const Scale s = row_scale(reduce.max_bits(m));
+    float m = 0.f;
+    for (int c = t; c < d; c += blockDim.x) m = max_abs(m, coded(c, value(c)));
+    const Scale s = row_scale(reduce.max_bits(__float_as_uint(m)));
     for (int c = t; c < d; c += blockDim.x) {
         const float v = value(c);
         p.out[row * p.out_ld + c] = (int8_t)code(coded(c, v), s);
@@ -363,7 +390,7 @@ static int launch_rows(const Args &p, cudaStream_t st) {
     if (p.d <= 32 * 48) row_kernel<T, MODE, true, 48, AL><<<(unsigned)(((int64_t)p.n + 3) / 4), 128, 0, st>>>(p);
     else if (p.d <= 128 * 16) launch_blocks<T, MODE, 16, AL>(p, st);
     else if (p.d <= 256 * 40) launch_blocks<T, MODE, 40, AL>(p, st);
-    else if (p.d <= 512 * 48) launch_blocks<T, MODE, 48, AL>(p, st);
+    else if (p.d <= 512 * 48) launch_blocks<T, MODE, sizeof(T) == 4 ? 24 : 48, AL>(p, st);   // registers
     else long_row_kernel<T, MODE><<<p.n, 512, 0, st>>>(p);
     return (int)cudaGetLastError();
 }
