@@ -254,17 +254,39 @@ kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtenso
                 tmem_wait_ld();
                 tmem_ld_fence32(v);
                 if constexpr (DT == SS_F32) {
-                    // thread = channel: a warp store covers 32 channels of a token, 128 bytes
+                    // thread = channel; half of the tokens at a time through shared memory, so that lane l
+                    // stores channels 4 (l % 8) .. + 4 of a token
 #pragma unroll
-                    for (int j = 0; j < 32; j += 2) {
-                        const uint64_t y = finish<GELU>(__float_as_int(v[j]), __float_as_int(v[j + 1]),
-                                                        f2_mul(f2(xs_s[j], xs_s[j + 1]), f2(wsv[0], wsv[0])),
-                                                        f2(bv[0], bv[0]));
-                        if (nw + lane < p.N) {
-                            float *dst = static_cast<float *>(p.out) + (mc + j) * p.out_ld + nw + lane;
-                            if (j < rows) dst[0] = f2_lo(y);
-                            if (j + 1 < rows) dst[p.out_ld] = f2_hi(y);
+                    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                        for (int j = 0; j < 16; j += 2) {
+                            const float2 x2 = *reinterpret_cast<const float2 *>(xs_s + 16 * h + j);
+                            const uint64_t y = finish<GELU>(__float_as_int(v[16 * h + j]), __float_as_int(v[16 * h + j + 1]),
+                                                            f2_mul(f2(x2.x, x2.y), f2(wsv[0], wsv[0])), f2(bv[0], bv[0]));
+                            asm volatile("st.shared.f32 [%0], %1;" ::"r"(turn + 128u * j + 4u * lane), "f"(f2_lo(y)) : "memory");
+                            asm volatile("st.shared.f32 [%0], %1;" ::"r"(turn + 128u * (j + 1) + 4u * lane), "f"(f2_hi(y)) : "memory");
                         }
+                        __syncwarp();
+                        const int nc = nw + 4 * (lane & 7);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int at = 4 * i + (lane >> 3), tok = 16 * h + at;
+                            float u[4];
+                            asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                         : "=f"(u[0]), "=f"(u[1]), "=f"(u[2]), "=f"(u[3])
+                                         : "r"(turn + 128u * at + 16u * (lane & 7)) : "memory");
+                            if (tok < rows) {
+                                float *dst = static_cast<float *>(p.out) + (mc + tok) * p.out_ld + nc;
+                                if (p.vec && nc + 3 < p.N) {
+                                    *reinterpret_cast<float4 *>(dst) = make_float4(u[0], u[1], u[2], u[3]);
+                                } else {
+#pragma unroll
+                                    for (int j = 0; j < 4; ++j)
+                                        if (nc + j < p.N) dst[j] = u[j];
+                                }
+                            }
+                        }
+                        __syncwarp();
                     }
                 } else {
                 // v[16 h + 4 i + 2 e + t]: channel 16 h + 8 e + lane / 4, token 8 i + 2 (lane % 4) + t
@@ -406,12 +428,18 @@ namespace split {
 constexpr int THREADS = 192;   // warps 0-3: accumulator rows; 4: TMA; 5: MMA; all: the final rows
 constexpr int MAX_TN = 128;
 constexpr int MAX_S = 8;
-enum Bar { FULL = 0, EMPTY = FULL + STAGES, ACC = EMPTY + STAGES, DRAIN = ACC + 1, NBAR = DRAIN + 1 };
+constexpr int MAX_STAGES = 5;
+enum Bar { FULL = 0, EMPTY = FULL + MAX_STAGES, ACC = EMPTY + MAX_STAGES, DRAIN = ACC + 1, NBAR = DRAIN + 1 };
 
 __host__ __device__ constexpr uint32_t stage_bytes(int tn) { return W_BYTES + (uint32_t)tn * BK; }
-__host__ __device__ constexpr uint32_t off_bar(int tn) { return STAGES * stage_bytes(tn); }
+// as many stages as leave room for two CTAs on an SM: a cluster of CTAs that each fill an SM leaves
+// SMs idle where a GPC's SMs are no multiple of it
+__host__ __device__ constexpr int stages(int tn) { return tn <= 32 ? 5 : tn <= 64 ? 4 : 3; }
+__host__ __device__ constexpr uint32_t off_bar(int tn) { return stages(tn) * stage_bytes(tn); }
 __host__ __device__ constexpr uint32_t smem_bytes(int tn) { return off_bar(tn) + NBAR * 8 + 32 + 1024; }
-static_assert(STAGES * W_BYTES >= 128u * 128u * 4u, "the sums fit in the stages' memory");
+constexpr uint32_t MAX_SMEM = smem_bytes(32);
+static_assert(MAX_SMEM >= smem_bytes(64) && MAX_SMEM >= smem_bytes(MAX_TN), "the largest of all tiles");
+static_assert(off_bar(MAX_TN) >= MAX_TN * 512u && off_bar(64) >= 64 * 512u, "the sums fit in the stages' memory");
 
 template <int DT, bool GELU>
 __global__ void __launch_bounds__(THREADS)
@@ -429,6 +457,7 @@ kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtenso
     const int m0 = (tile / p.ncb) * p.tn;
     const int nk = (p.K + BK - 1) / BK;
     const int k_lo = (int)((int64_t)rank * nk / S), k_hi = (int)((int64_t)(rank + 1) * nk / S);
+    const int nst = stages(p.tn);
     const uint32_t cols = p.tn <= 32 ? 32u : p.tn <= 64 ? 64u : 128u;
 
     if (tid == 0) {
@@ -453,9 +482,9 @@ kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtenso
         const uint32_t bytes = stage_bytes(p.tn);
         int i = 0;
         for (int k = k_lo; k < k_hi; ++k, ++i) {
-            const int st = i % STAGES;
-            if (i >= STAGES) {
-                ok = warp_all(mbar_wait(bar(EMPTY + st), (i / STAGES - 1) & 1, abort_flag));
+            const int st = i % nst;
+            if (i >= nst) {
+                ok = warp_all(mbar_wait(bar(EMPTY + st), (i / nst - 1) & 1, abort_flag));
                 if (!ok) break;
             }
             if (elect_one()) {
@@ -468,13 +497,13 @@ kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtenso
         }
         if (!ok) report(p.status, SS_DEV_TIMEOUT);
         if (!ok || *abort_flag)
-            for (int s = i > STAGES ? i - STAGES : 0; s < i; ++s) drain_wait(bar(FULL + s % STAGES), (s / STAGES) & 1);
+            for (int s = i > nst ? i - nst : 0; s < i; ++s) drain_wait(bar(FULL + s % nst), (s / nst) & 1);
     } else if (warp == 5) {
         const uint32_t idesc = idesc_i8(128, p.tn), bytes = stage_bytes(p.tn);
         int i = 0;
         for (int k = k_lo; k < k_hi; ++k, ++i) {
-            const int st = i % STAGES;
-            ok = warp_all(mbar_wait(bar(FULL + st), (i / STAGES) & 1, abort_flag));
+            const int st = i % nst;
+            ok = warp_all(mbar_wait(bar(FULL + st), (i / nst) & 1, abort_flag));
             if (!ok) break;
             tc_fence_after();
             const uint64_t da = smem_desc_sw128(sbase + (uint32_t)st * bytes, 16, 1024);
@@ -568,6 +597,94 @@ kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtenso
 
 }  // namespace split
 
+// ---------------------------------------------------------------------------------------------
+// one to four tokens: dot products
+// ---------------------------------------------------------------------------------------------
+// The weights are read once, straight to registers, 16 bytes a lane; WPC warps of a block share a
+// group of CH channels, each taking every WPC-th 512 bytes of their rows. Lanes' sums meet by
+// redux, warps' through shared memory. Bytes past K of a row's last 16 count as 0 through x.
+namespace dot {
+
+constexpr int WARPS = 8;
+
+template <int DT, bool GELU, int MT, int CH, int WPC>
+__global__ void __launch_bounds__(WARPS * 32)
+kernel(const int8_t *__restrict__ x, int64_t x_ld, const int8_t *__restrict__ w, int64_t w_ld, const Params p) {
+    __shared__ int red[WARPS][CH * MT];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % WPC;
+    const int n0 = (blockIdx.x * (WARPS / WPC) + warp / WPC) * CH;
+    const int chunks = (p.K + 15) / 16;
+    const uint4 *wr[CH];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) wr[c] = reinterpret_cast<const uint4 *>(w + (int64_t)min(n0 + c, p.N - 1) * w_ld);
+    int acc[CH][MT] = {};
+#pragma unroll 4
+    for (int k = part * 32 + lane; k < chunks; k += WPC * 32) {
+        uint4 a[CH];
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+            asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(a[c].x), "=r"(a[c].y), "=r"(a[c].z), "=r"(a[c].w) : "l"(wr[c] + k));
+        const int left = p.K - 16 * k;   // codes of this chunk that are the row's
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            uint4 b = reinterpret_cast<const uint4 *>(x + (int64_t)min(m, p.M - 1) * x_ld)[k];
+            if (left < 16) {
+                uint32_t *e = &b.x;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    e[j] &= left >= 4 * j + 4 ? ~0u : left <= 4 * j ? 0u : (1u << (8 * (left - 4 * j))) - 1u;
+            }
+#pragma unroll
+            for (int c = 0; c < CH; ++c) {
+                acc[c][m] = __dp4a((int)a[c].x, (int)b.x, acc[c][m]);
+                acc[c][m] = __dp4a((int)a[c].y, (int)b.y, acc[c][m]);
+                acc[c][m] = __dp4a((int)a[c].z, (int)b.z, acc[c][m]);
+                acc[c][m] = __dp4a((int)a[c].w, (int)b.w, acc[c][m]);
+            }
+        }
+    }
+    int mine = 0;   // lane c MT + m keeps the sum of channel c and token m
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            const int t = __reduce_add_sync(0xffffffffu, acc[c][m]);
+            if (lane == c * MT + m) mine = t;
+        }
+    if (WPC > 1) {
+        if (lane < CH * MT) red[warp][lane] = mine;
+        __syncthreads();
+        if (part != 0) return;
+        if (lane < CH * MT)
+#pragma unroll
+            for (int i = 1; i < WPC; ++i) mine += red[warp + i][lane];
+    }
+    const int n = n0 + lane / MT, m = lane % MT;
+    if (lane < CH * MT && n < p.N && m < p.M) {
+        const float s = __fmul_rn(p.xs[m], p.ws[n]), b = p.bias ? load_any(p.bias, p.bias_dtype, n) : 0.f;
+        store_one<DT>(p.out, m * p.out_ld + n, f2_lo(finish<GELU>(mine, 0, f2(s, 0.f), f2(b, 0.f))));
+    }
+}
+
+template <int DT, bool GELU, int MT, int CH>
+static int launch(const int8_t *x, int64_t x_ld, const int8_t *w, int64_t w_ld, const Params &p, int nsm,
+                  cudaStream_t st) {
+    // enough warps for 16 an SM, as long as each has 512 bytes of a row to read
+    const int64_t groups = (p.N + CH - 1) / CH;
+    const int steps = (p.K + 511) / 512;
+    int wpc = 1;
+    while (wpc < WARPS && groups * wpc < 16 * (int64_t)nsm && wpc * 2 <= steps) wpc *= 2;
+    const unsigned blocks = (unsigned)((groups * wpc + WARPS - 1) / WARPS);
+    if (wpc == 1) kernel<DT, GELU, MT, CH, 1><<<blocks, WARPS * 32, 0, st>>>(x, x_ld, w, w_ld, p);
+    else if (wpc == 2) kernel<DT, GELU, MT, CH, 2><<<blocks, WARPS * 32, 0, st>>>(x, x_ld, w, w_ld, p);
+    else if (wpc == 4) kernel<DT, GELU, MT, CH, 4><<<blocks, WARPS * 32, 0, st>>>(x, x_ld, w, w_ld, p);
+    else kernel<DT, GELU, MT, CH, 8><<<blocks, WARPS * 32, 0, st>>>(x, x_ld, w, w_ld, p);
+    return (int)cudaGetLastError();
+}
+
+}  // namespace dot
+
 static bool off(const void *p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) != 0; }
 static size_t type_bytes(int dtype) { return dtype == SS_F32 ? 4 : 2; }
 static bool known(int dtype) { return dtype == SS_BF16 || dtype == SS_F32 || dtype == SS_F16; }
@@ -585,7 +702,7 @@ static cudaError_t linear_i8_attributes() {
                                          (int)lin::pair::SMEM_BYTES);
     if (e != cudaSuccess) return e;
     return cudaFuncSetAttribute(lin::split::kernel<DT, GELU>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                (int)lin::split::smem_bytes(lin::split::MAX_TN));
+                                (int)lin::split::MAX_SMEM);
 }
 
 int linear_i8_prepare(int device) {
@@ -641,6 +758,9 @@ static Plan choose(int M, int N, int K, int nsm) {
 template <int DT, bool GELU>
 static int launch(const Plan &plan, const int8_t *x, int64_t x_ld, const int8_t *w, int64_t w_ld, Params p, int nsm,
                   cudaStream_t st) {
+    if (p.M == 1) return dot::launch<DT, GELU, 1, 2>(x, x_ld, w, w_ld, p, nsm, st);
+    if (p.M == 2) return dot::launch<DT, GELU, 2, 2>(x, x_ld, w, w_ld, p, nsm, st);
+    if (p.M <= 4) return dot::launch<DT, GELU, 4, 2>(x, x_ld, w, w_ld, p, nsm, st);
     CUtensorMap tm_w, tm_x;
     p.tn = plan.tn;
     int rc = encode_tmap_2d_u8(&tm_w, w, (uint64_t)p.K, (uint64_t)p.N, (uint64_t)w_ld, BK, 128);

@@ -852,13 +852,19 @@ LINEAR_I8_MAX_K = 131071
 def _no_grad(*tensors) -> None:
     if torch.is_grad_enabled():
         for t in tensors:
-            _require(t is None or not t.requires_grad, "the 8-bit linear path has no gradient: call it under "
-                                                       "torch.no_grad() or detach its inputs")
+            if t is not None and t.requires_grad:
+                raise ValueError("the 8-bit linear path has no gradient: call it under torch.no_grad() or detach its "
+                                 "inputs")
+
+
+def _stream_handle(device) -> int:
+    """The current stream's handle of a tensor's device, without building a stream object."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def _ld(t: torch.Tensor, name: str, n: int, d: int, dtype: torch.dtype, device) -> int:
     """Row stride of t [n, d] (the values of a row contiguous, the rows at any stride of at least d)."""
-    if t.dtype != dtype or t.dim() != 2 or t.shape[0] != n or t.shape[1] != d or t.device != device:
+    if t.dtype != dtype or t.shape != (n, d) or t.device != device:
         raise ValueError(f"{name}: expected {dtype} [{n}, {d}] on {device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
     ld, step = t.stride()
     if n <= 1:
@@ -877,10 +883,11 @@ def _vec(t: torch.Tensor, name: str, d: int, dtype: torch.dtype, device) -> int:
 def _frame_rows(t: torch.Tensor, name: str, n: int, d: int, frame_tokens: int, device) -> int:
     if t.dtype != torch.float32 or t.dim() != 2 or t.shape[1] != d or t.device != device:
         raise ValueError(f"{name}: fp32 [frames, {d}] on {device} expected")
-    if frame_tokens <= 0 or t.shape[0] * frame_tokens < n:
+    frames = t.shape[0]
+    if frame_tokens <= 0 or frames * frame_tokens < n:
         raise ValueError("frame_tokens must cover the rows")
     ld, step = t.stride()
-    if t.shape[0] <= 1:
+    if frames <= 1:
         ld = d
     if (step != 1 and d != 1) or ld < d:
         raise ValueError(f"{name}: rows of {d} contiguous values that do not overlap expected")
@@ -897,7 +904,7 @@ def rows_i8(n: int, d: int, device) -> torch.Tensor:
 def _rows_i8_in(x: torch.Tensor, name: str):
     if not x.is_cuda or x.dim() != 2 or x.dtype not in _I8_TYPES or x.shape[1] < 1:
         raise ValueError(f"{name}: CUDA tensor [n, d >= 1] of bfloat16, float16 or float32 expected")
-    return x.shape[0], x.shape[1], x.dtype, x.device
+    return *x.shape, x.dtype, x.device
 
 
 def _rows_i8_out(out, scales, n: int, d: int, device):
@@ -924,9 +931,24 @@ def quant_rows(x: torch.Tensor, *, out: torch.Tensor | None = None, scales: torc
     x_ld = _ld(x, "x", n, d, dtype, dev)
     out, o_ld, scales = _rows_i8_out(out, scales, n, d, dev)
     rc = lib().ss_quant_rows(x.data_ptr(), x_ld, _I8_TYPES[dtype], n, d, out.data_ptr(), o_ld, scales.data_ptr(),
-                             _stream(dev))
-    check(rc, "ss_quant_rows")
+                             _stream_handle(dev))
+    if rc:
+        check(rc, "ss_quant_rows")
     return out, scales
+
+
+def _residual(residual, sum_out, name: str, n: int, d: int, dtype, dev):
+    """(residual pointer, its row stride, sum buffer, its pointer and row stride); the sum goes with a residual."""
+    if residual is None:
+        if sum_out is not None:
+            raise ValueError(f"sum_out goes with {name}")
+        return None, 0, None, None, 0
+    r_ld = _ld(residual, name, n, d, dtype, dev)
+    if sum_out is None:
+        sum_out, s_ld = torch.empty_like(residual, memory_format=torch.contiguous_format), d
+    else:
+        s_ld = _ld(sum_out, "sum_out", n, d, dtype, dev)
+    return residual.data_ptr(), r_ld, sum_out, sum_out.data_ptr(), s_ld
 
 
 def rms_norm_i8(x: torch.Tensor, weight: torch.Tensor, eps: float, *, residual: torch.Tensor | None = None,
@@ -943,24 +965,13 @@ def rms_norm_i8(x: torch.Tensor, weight: torch.Tensor, eps: float, *, residual: 
     _no_grad(x, weight, residual)
     x_ld = _ld(x, "x", n, d, dtype, dev)
     w = _vec(weight, "weight", d, dtype, dev)
-    r, r_ld, s, s_ld = _residual(residual, sum_out, "residual", n, d, dtype, dev)
+    r, r_ld, s, sp, s_ld = _residual(residual, sum_out, "residual", n, d, dtype, dev)
     out, o_ld, scales = _rows_i8_out(out, scales, n, d, dev)
-    rc = lib().ss_rms_norm_i8(x.data_ptr(), x_ld, r, r_ld, _I8_TYPES[dtype], n, d, w, float(eps),
-                              None if s is None else s.data_ptr(), s_ld, out.data_ptr(), o_ld, scales.data_ptr(),
-                              _stream(dev))
-    check(rc, "ss_rms_norm_i8")
+    rc = lib().ss_rms_norm_i8(x.data_ptr(), x_ld, r, r_ld, _I8_TYPES[dtype], n, d, w, eps, sp, s_ld, out.data_ptr(),
+                              o_ld, scales.data_ptr(), _stream_handle(dev))
+    if rc:
+        check(rc, "ss_rms_norm_i8")
     return (out, scales) if s is None else (out, scales, s)
-
-
-def _residual(residual, sum_out, name: str, n: int, d: int, dtype, dev):
-    """(residual pointer, its row stride, sum buffer, its row stride); the sum goes with a residual."""
-    if residual is None:
-        _require(sum_out is None, f"sum_out goes with {name}")
-        return None, 0, None, 0
-    r_ld = _ld(residual, name, n, d, dtype, dev)
-    if sum_out is None:
-        return residual.data_ptr(), r_ld, torch.empty((n, d), dtype=dtype, device=dev), d
-    return residual.data_ptr(), r_ld, sum_out, _ld(sum_out, "sum_out", n, d, dtype, dev)
 
 
 def adaln_i8(x: torch.Tensor, *, eps: float, shift: torch.Tensor | None = None, scale: torch.Tensor | None = None,
@@ -978,28 +989,28 @@ def adaln_i8(x: torch.Tensor, *, eps: float, shift: torch.Tensor | None = None, 
     n, d, dtype, dev = _rows_i8_in(x, "x")
     _no_grad(x, shift, scale, weight, bias, y, gate)
     x_ld = _ld(x, "x", n, d, dtype, dev)
-    m = [None, None, None, None]
+    if (shift is None) != (scale is None) or (weight is None) != (bias is None) or (shift is None) == (weight is None):
+        raise ValueError("give shift and scale, or weight and bias")
+    shp = scp = wp = bp = gp = None
     mod_ld = g_ld = 0
-    if weight is not None or bias is not None:
-        _require(weight is not None and bias is not None, "weight and bias go together")
-        _require(shift is None and scale is None, "give shift and scale, or weight and bias")
-        m[2], m[3] = _vec(weight, "weight", d, dtype, dev), _vec(bias, "bias", d, dtype, dev)
+    if weight is not None:
+        wp, bp = _vec(weight, "weight", d, dtype, dev), _vec(bias, "bias", d, dtype, dev)
     else:
-        _require(shift is not None and scale is not None, "give shift and scale, or weight and bias")
         mod_ld = _frame_rows(shift, "shift", n, d, frame_tokens, dev)
-        _require(_frame_rows(scale, "scale", n, d, frame_tokens, dev) == mod_ld,
-                 "shift and scale must share a row stride")
-        m[0], m[1] = shift.data_ptr(), scale.data_ptr()
+        if _frame_rows(scale, "scale", n, d, frame_tokens, dev) != mod_ld:
+            raise ValueError("shift and scale must share a row stride")
+        shp, scp = shift.data_ptr(), scale.data_ptr()
     if gate is not None:
-        _require(y is not None, "gate goes with y")
-        g_ld = _frame_rows(gate, "gate", n, d, frame_tokens, dev)
-    r, r_ld, s, s_ld = _residual(y, sum_out, "y", n, d, dtype, dev)
+        if y is None:
+            raise ValueError("gate goes with y")
+        g_ld, gp = _frame_rows(gate, "gate", n, d, frame_tokens, dev), gate.data_ptr()
+    r, r_ld, s, sp, s_ld = _residual(y, sum_out, "y", n, d, dtype, dev)
     out, o_ld, scales = _rows_i8_out(out, scales, n, d, dev)
-    rc = lib().ss_adaln_i8(x.data_ptr(), x_ld, r, r_ld, None if gate is None else gate.data_ptr(), g_ld,
-                           _I8_TYPES[dtype], n, d, int(frame_tokens), m[0], m[1], mod_ld, m[2], m[3], float(eps),
-                           None if s is None else s.data_ptr(), s_ld, out.data_ptr(), o_ld, scales.data_ptr(),
-                           _stream(dev))
-    check(rc, "ss_adaln_i8")
+    rc = lib().ss_adaln_i8(x.data_ptr(), x_ld, r, r_ld, gp, g_ld, _I8_TYPES[dtype], n, d, frame_tokens, shp, scp,
+                           mod_ld, wp, bp, eps, sp, s_ld, out.data_ptr(), o_ld, scales.data_ptr(),
+                           _stream_handle(dev))
+    if rc:
+        check(rc, "ss_adaln_i8")
     return (out, scales) if s is None else (out, scales, s)
 
 
@@ -1034,13 +1045,15 @@ def linear_i8(x_i8: torch.Tensor, xs: torch.Tensor, w_i8: torch.Tensor, ws: torc
             raise ValueError("out_dtype: bfloat16, float16 or float32 expected")
         out, o_ld = torch.empty((M, N), dtype=out_dtype, device=dev), N
     else:
-        _require(out.dtype in _I8_TYPES, "out: bfloat16, float16 or float32 expected")
-        o_ld = _ld(out, "out", M, N, out.dtype, dev)
-    status = DeviceStatus.word(dev)
-    rc = lib().ss_linear_i8(xp, x_ld, xsp, wp, w_ld, wsp, bp, 0 if bias is None else _I8_TYPES[bias.dtype],
-                            int(gelu), M, N, K, out.data_ptr(), o_ld, _I8_TYPES[out.dtype], status.data_ptr(),
-                            _stream(dev))
-    check(rc, "ss_linear_i8")
+        out_dtype = out.dtype
+        if out_dtype not in _I8_TYPES:
+            raise ValueError("out: bfloat16, float16 or float32 expected")
+        o_ld = _ld(out, "out", M, N, out_dtype, dev)
+    rc = lib().ss_linear_i8(xp, x_ld, xsp, wp, w_ld, wsp, bp, 0 if bias is None else _I8_TYPES[bias.dtype], bool(gelu),
+                            M, N, K, out.data_ptr(), o_ld, _I8_TYPES[out_dtype], DeviceStatus.word(dev).data_ptr(),
+                            _stream_handle(dev))
+    if rc:
+        check(rc, "ss_linear_i8")
     if validate:
         DeviceStatus.check(dev)
     return out
