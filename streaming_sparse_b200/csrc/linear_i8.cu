@@ -155,9 +155,31 @@ __device__ __forceinline__ bool drain_wait(uint32_t bar, uint32_t parity) {
     return true;
 }
 
+// a place in a ring of n stages and the parity of its barriers there (no division: it is on the
+// critical path of every step)
+struct Ring {
+    int n, at = 0;
+    uint32_t parity = 0;
+    __device__ __forceinline__ void next() {
+        if (++at == n) {
+            at = 0;
+            parity ^= 1u;
+        }
+    }
+    // the j-th stage before this one, j <= n
+    __device__ __forceinline__ Ring before(int j) const {
+        Ring r = *this;
+        r.at -= j;
+        if (r.at < 0) {
+            r.at += n;
+            r.parity ^= 1u;
+        }
+        return r;
+    }
+};
+
 constexpr int BK = 128;                          // codes a stage: one 128-byte swizzled row
 constexpr uint32_t W_BYTES = 128 * BK;           // 128 channels of a stage
-constexpr int STAGES = 6;
 
 // ---------------------------------------------------------------------------------------------
 // many tokens: an SM pair per tile of 256 channels x tn tokens
@@ -170,15 +192,18 @@ namespace pair {
 
 constexpr int EPI_WARPS = 8;
 constexpr int THREADS = (EPI_WARPS + 2) * 32;
-constexpr uint32_t X_BYTES = 128 * BK;           // half of 256 tokens
-constexpr uint32_t STAGE_BYTES = W_BYTES + X_BYTES;
-constexpr uint32_t OFF_TURN = STAGES * STAGE_BYTES;            // per epilogue warp: 32 tokens x 32 channels of 16 bits
+constexpr uint32_t RING_BYTES = 6 * 2 * W_BYTES;               // six stages of the largest tile
+constexpr int MAX_STAGES = 10;
+constexpr uint32_t OFF_TURN = RING_BYTES;                      // per epilogue warp: 32 tokens x 32 channels of 16 bits
 constexpr uint32_t OFF_BAR = OFF_TURN + EPI_WARPS * 2048;
-enum Bar { FULL = 0, EMPTY = FULL + STAGES, ACC_FULL = EMPTY + STAGES, ACC_EMPTY = ACC_FULL + 2,
+enum Bar { FULL = 0, EMPTY = FULL + MAX_STAGES, ACC_FULL = EMPTY + MAX_STAGES, ACC_EMPTY = ACC_FULL + 2,
            DRAIN = ACC_EMPTY + 2, NBAR = DRAIN + 1 };
 constexpr uint32_t OFF_MISC = OFF_BAR + NBAR * 8 + (NBAR % 2) * 8;   // [0] tmem, [1] abort
 constexpr uint32_t OFF_XS = OFF_MISC + 16;
-constexpr uint32_t SMEM_BYTES = OFF_XS + EPI_WARPS * 32 * 4 + 1024;         // + alignment slack
+constexpr uint32_t SMEM_BYTES = OFF_XS + EPI_WARPS * 128 * 4 + 1024;         // + alignment slack
+
+__host__ __device__ constexpr uint32_t stage_bytes(int tn) { return W_BYTES + (uint32_t)(tn / 2) * BK; }
+// a smaller tile's stages are smaller, and its loop waits for the loads' latency: more of them fit
 
 template <int DT, bool GELU>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
@@ -194,6 +219,8 @@ kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtenso
     const uint32_t rank = cluster_rank();
     const int pair_id = blockIdx.x >> 1, npairs = gridDim.x >> 1;
     const int nk = (p.K + BK - 1) / BK;
+    const uint32_t stage = stage_bytes(p.tn);
+    const int nst = min((int)(RING_BYTES / stage), MAX_STAGES);
 
     if (tid == 0) {
         for (int i = 0; i < NBAR; ++i)
@@ -219,7 +246,7 @@ kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtenso
         const int wg = warp >> 2;
         const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
         const uint32_t acc_empty = in_cta(bar(ACC_EMPTY), 0);
-        float *xs_s = reinterpret_cast<float *>(smem + OFF_XS) + warp * 32;   // the chunk's token scales
+        float *xs_w = reinterpret_cast<float *>(smem + OFF_XS) + warp * 128;   // the tile's token scales
         const uint32_t turn = sbase + OFF_TURN + (uint32_t)warp * 2048;
         bool ok = true;
         int it = 0;
@@ -234,25 +261,32 @@ kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtenso
                 wsv[i] = n < p.N ? p.ws[n] : 0.f;
                 bv[i] = (p.bias && n < p.N) ? load_any(p.bias, p.bias_dtype, n) : 0.f;
             }
+            // the scales of the warp's tokens: 32-token chunks wg, wg + 2, ... of the tile
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int64_t m = m0 + 32 * (2 * i + wg) + lane;
+                if (32 * (2 * i + wg) < p.tn) xs_w[32 * i + lane] = m < p.M ? p.xs[m] : 0.f;
+            }
+            __syncwarp();
             const int b = it & 1;
             ok = warp_all(mbar_wait(bar(ACC_FULL + b), (it >> 1) & 1, abort_flag));
             if (!ok) break;
             tc_fence_after();
-            for (int c = wg; c < p.tn / 32; c += 2) {
+            const uint32_t acc = lanes + 256 * b;
+            auto load = [&](int c, float (&v)[32]) {
+                if (DT == SS_F32) {
+                    tmem_ld32(acc + 32 * c, v);
+                } else {   // 16 channels x 32 tokens twice, as 8 x 8 fragments
+                    tmem_ld_16x256b_x4(acc + 32 * c, v);
+                    tmem_ld_16x256b_x4(acc + 32 * c + (16u << 16), v + 16);
+                }
+            };
+            auto store = [&](int c, float (&v)[32]) {
                 const int64_t mc = m0 + 32 * c;
                 const int rows = (int)min((int64_t)32, p.M - mc);
-                float v[32];
-                if (DT == SS_F32) {
-                    tmem_ld32(lanes + 256 * b + 32 * c, v);
-                } else {   // 16 channels x 32 tokens twice, as 8 x 8 fragments
-                    tmem_ld_16x256b_x4(lanes + 256 * b + 32 * c, v);
-                    tmem_ld_16x256b_x4(lanes + 256 * b + 32 * c + (16u << 16), v + 16);
-                }
+                const float *xs_s = xs_w + 16 * (c - wg);
                 __syncwarp();   // the chunk before has left the warp's shared memory
-                xs_s[lane] = lane < rows ? p.xs[mc + lane] : 0.f;
-                __syncwarp();
-                tmem_wait_ld();
-                tmem_ld_fence32(v);
                 if constexpr (DT == SS_F32) {
                     // thread = channel; half of the tokens at a time through shared memory, so that lane l
                     // stores channels 4 (l % 8) .. + 4 of a token
@@ -333,6 +367,22 @@ kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtenso
                     }
                 }
                 }
+            };
+            // the next chunk comes out of TMEM while this one is finished and stored
+            const int nc = p.tn / 32;
+            float v0[32], v1[32];
+            if (wg < nc) load(wg, v0);
+            for (int c = wg; c < nc; c += 4) {
+                tmem_wait_ld();
+                tmem_ld_fence32(v0);
+                if (c + 2 < nc) load(c + 2, v1);
+                store(c, v0);
+                if (c + 2 < nc) {
+                    tmem_wait_ld();
+                    tmem_ld_fence32(v1);
+                    if (c + 4 < nc) load(c + 4, v0);
+                    store(c + 2, v1);
+                }
             }
             tc_fence_before();
             __syncwarp();
@@ -343,60 +393,62 @@ kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtenso
         // ---------------- TMA producer (both CTAs) ----------------
         const uint32_t x_bytes = (uint32_t)(p.tn / 2) * BK;
         const uint32_t full = in_cta(bar(FULL), 0);
-        int i = 0;   // stages issued
+        Ring ring{nst};
+        int issued = 0;
         bool ok = true;
         for (int tile = pair_id; tile < p.ntiles && ok; tile += npairs) {
             const int n0 = (tile % p.ncb) * 256 + (int)rank * 128;
             const int m0 = (tile / p.ncb) * p.tn + (int)rank * (p.tn / 2);
-            for (int k = 0; k < nk; ++k, ++i) {
-                const int st = i % STAGES;
-                if (i >= STAGES) {
-                    ok = warp_all(mbar_wait(bar(EMPTY + st), (i / STAGES - 1) & 1, abort_flag));
-                    if (!ok) break;
-                }
+            for (int k = 0; k < nk; ++k) {
+                // a fresh barrier counts as released: the first round does not wait
+                ok = warp_all(mbar_wait(bar(EMPTY + ring.at), ring.parity ^ 1u, abort_flag));
+                if (!ok) break;
                 if (elect_one()) {
-                    const uint32_t dst = sbase + (uint32_t)st * STAGE_BYTES;
-                    if (rank == 0) mbar_arrive_expect_tx(bar(FULL + st), 2 * (W_BYTES + x_bytes));
-                    tma_load_2d_pair(dst, &tm_w, k * BK, n0, full + 8u * (uint32_t)st);
-                    tma_load_2d_pair(dst + W_BYTES, &tm_x, k * BK, m0, full + 8u * (uint32_t)st);
+                    const uint32_t dst = sbase + (uint32_t)ring.at * stage;
+                    if (rank == 0) mbar_arrive_expect_tx(bar(FULL + ring.at), 2 * (W_BYTES + x_bytes));
+                    tma_load_2d_pair(dst, &tm_w, k * BK, n0, full + 8u * (uint32_t)ring.at);
+                    tma_load_2d_pair(dst + W_BYTES, &tm_x, k * BK, m0, full + 8u * (uint32_t)ring.at);
                 }
                 __syncwarp();
+                ring.next();
+                issued = min(issued + 1, nst);
             }
         }
         if (!ok) report(p.status, SS_DEV_TIMEOUT);
         if (!ok || *abort_flag) {
             // the loads still in flight land before the CTA's shared memory goes away: the even CTA sees
             // both CTAs' by its full barriers, the odd one only by the stages' release
-            for (int s = i > STAGES ? i - STAGES : 0; s < i; ++s)
-                drain_wait(bar((rank == 0 ? FULL : EMPTY) + s % STAGES), (s / STAGES) & 1);
+            for (int j = issued; j > 0; --j) {
+                const Ring r = ring.before(j);
+                drain_wait(bar((rank == 0 ? FULL : EMPTY) + r.at), r.parity);
+            }
         }
     } else if (rank == 0) {
         // ---------------- MMA issuer (the even CTA) ----------------
         const uint32_t idesc = idesc_i8(256, p.tn);
-        int i = 0, it = 0;
+        const uint64_t dw = smem_desc_sw128(sbase, 16, 1024), dx = smem_desc_sw128(sbase + W_BYTES, 16, 1024);
+        Ring ring{nst};
+        int it = 0;
         bool ok = true;
         for (int tile = pair_id; tile < p.ntiles && ok; tile += npairs, ++it) {
             const int b = it & 1;
-            if (it >= 2) {
-                ok = warp_all(mbar_wait(bar(ACC_EMPTY + b), ((it >> 1) - 1) & 1, abort_flag));
-                if (!ok) break;
-            }
+            ok = warp_all(mbar_wait(bar(ACC_EMPTY + b), ((it >> 1) & 1) ^ 1, abort_flag));
+            if (!ok) break;
             tc_fence_after();
-            for (int k = 0; k < nk; ++k, ++i) {
-                const int st = i % STAGES;
-                ok = warp_all(mbar_wait(bar(FULL + st), (i / STAGES) & 1, abort_flag));
+            for (int k = 0; k < nk; ++k) {
+                ok = warp_all(mbar_wait(bar(FULL + ring.at), ring.parity, abort_flag));
                 if (!ok) break;
                 tc_fence_after();
-                const uint64_t da = smem_desc_sw128(sbase + (uint32_t)st * STAGE_BYTES, 16, 1024);
-                const uint64_t db = smem_desc_sw128(sbase + (uint32_t)st * STAGE_BYTES + W_BYTES, 16, 1024);
+                const uint64_t to = (uint64_t)((uint32_t)ring.at * stage >> 4);
                 if (elect_one()) {
 #pragma unroll
                     for (int kk = 0; kk < BK / 32; ++kk)
-                        mma_i8<2>(tmem + 256 * b, da + 2 * kk, db + 2 * kk, idesc, (k > 0 || kk > 0) ? 1u : 0u);
-                    commit_both(bar(EMPTY + st));
+                        mma_i8<2>(tmem + 256 * b, dw + to + 2 * kk, dx + to + 2 * kk, idesc, (k > 0 || kk > 0) ? 1u : 0u);
+                    commit_both(bar(EMPTY + ring.at));
                     if (k == nk - 1) commit_both(bar(ACC_FULL + b));
                 }
                 __syncwarp();
+                ring.next();
             }
         }
         if (!ok) report(p.status, SS_DEV_TIMEOUT);
@@ -441,9 +493,9 @@ constexpr uint32_t MAX_SMEM = smem_bytes(32);
 static_assert(MAX_SMEM >= smem_bytes(64) && MAX_SMEM >= smem_bytes(MAX_TN), "the largest of all tiles");
 static_assert(off_bar(MAX_TN) >= MAX_TN * 512u && off_bar(64) >= 64 * 512u, "the sums fit in the stages' memory");
 
-template <int DT, bool GELU>
+template <int DT, bool GELU, int S>
 __global__ void __launch_bounds__(THREADS)
-kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, const Params p, int S) {
+kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, const Params p) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const uint32_t sbase = smem_u32(smem);
@@ -480,42 +532,46 @@ kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtenso
 
     if (warp == 4) {
         const uint32_t bytes = stage_bytes(p.tn);
-        int i = 0;
-        for (int k = k_lo; k < k_hi; ++k, ++i) {
-            const int st = i % nst;
-            if (i >= nst) {
-                ok = warp_all(mbar_wait(bar(EMPTY + st), (i / nst - 1) & 1, abort_flag));
-                if (!ok) break;
-            }
+        Ring ring{nst};
+        int issued = 0;
+        for (int k = k_lo; k < k_hi; ++k) {
+            // a fresh barrier counts as released: the first round does not wait
+            ok = warp_all(mbar_wait(bar(EMPTY + ring.at), ring.parity ^ 1u, abort_flag));
+            if (!ok) break;
             if (elect_one()) {
-                const uint32_t dst = sbase + (uint32_t)st * bytes;
-                mbar_arrive_expect_tx(bar(FULL + st), bytes);
-                tma_load_2d(dst, &tm_w, k * BK, n0, bar(FULL + st));
-                tma_load_2d(dst + W_BYTES, &tm_x, k * BK, m0, bar(FULL + st));
+                const uint32_t dst = sbase + (uint32_t)ring.at * bytes;
+                mbar_arrive_expect_tx(bar(FULL + ring.at), bytes);
+                tma_load_2d(dst, &tm_w, k * BK, n0, bar(FULL + ring.at));
+                tma_load_2d(dst + W_BYTES, &tm_x, k * BK, m0, bar(FULL + ring.at));
             }
             __syncwarp();
+            ring.next();
+            issued = min(issued + 1, nst);
         }
         if (!ok) report(p.status, SS_DEV_TIMEOUT);
         if (!ok || *abort_flag)
-            for (int s = i > nst ? i - nst : 0; s < i; ++s) drain_wait(bar(FULL + s % nst), (s / nst) & 1);
+            for (int j = issued; j > 0; --j) {   // the loads in flight land before the shared memory goes away
+                const Ring r = ring.before(j);
+                drain_wait(bar(FULL + r.at), r.parity);
+            }
     } else if (warp == 5) {
         const uint32_t idesc = idesc_i8(128, p.tn), bytes = stage_bytes(p.tn);
-        int i = 0;
-        for (int k = k_lo; k < k_hi; ++k, ++i) {
-            const int st = i % nst;
-            ok = warp_all(mbar_wait(bar(FULL + st), (i / nst) & 1, abort_flag));
+        const uint64_t dw = smem_desc_sw128(sbase, 16, 1024), dx = smem_desc_sw128(sbase + W_BYTES, 16, 1024);
+        Ring ring{nst};
+        for (int k = k_lo; k < k_hi; ++k) {
+            ok = warp_all(mbar_wait(bar(FULL + ring.at), ring.parity, abort_flag));
             if (!ok) break;
             tc_fence_after();
-            const uint64_t da = smem_desc_sw128(sbase + (uint32_t)st * bytes, 16, 1024);
-            const uint64_t db = smem_desc_sw128(sbase + (uint32_t)st * bytes + W_BYTES, 16, 1024);
+            const uint64_t to = (uint64_t)((uint32_t)ring.at * bytes >> 4);
             if (elect_one()) {
 #pragma unroll
                 for (int kk = 0; kk < BK / 32; ++kk)
-                    mma_i8<1>(tmem, da + 2 * kk, db + 2 * kk, idesc, (i > 0 || kk > 0) ? 1u : 0u);
-                tc_commit(bar(EMPTY + st));
+                    mma_i8<1>(tmem, dw + to + 2 * kk, dx + to + 2 * kk, idesc, (k > k_lo || kk > 0) ? 1u : 0u);
+                tc_commit(bar(EMPTY + ring.at));
                 if (k == k_hi - 1) tc_commit(bar(ACC));
             }
             __syncwarp();
+            ring.next();
         }
         if (!ok) report(p.status, SS_DEV_TIMEOUT);
         if (!ok || *abort_flag) {
@@ -545,23 +601,28 @@ kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtenso
     else __syncthreads();
     // after a wait that ran out the sums are not whole, but the memory they are read from is there
     const int t_lo = rank * p.tn / S, t_hi = (rank + 1) * p.tn / S;
+    // each thread keeps its four channels: 32 threads a token
+#pragma unroll 2
     for (int i = tid; i < (t_hi - t_lo) * 32; i += THREADS) {
         const int t = t_lo + i / 32, c = (i % 32) * 4;
         const int64_t m = (int64_t)m0 + t;
         if (m >= p.M) break;
         const uint32_t at = sbase + (uint32_t)(t * 128 + c) * 4u;
-        int a[4] = {0, 0, 0, 0};
+        int b[S][4], a[4] = {0, 0, 0, 0};
+#pragma unroll
         for (int r = 0; r < S; ++r) {
-            int b[4];
             if (S > 1)
                 asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
-                             : "=r"(b[0]), "=r"(b[1]), "=r"(b[2]), "=r"(b[3]) : "r"(in_cta(at, (uint32_t)r)));
+                             : "=r"(b[r][0]), "=r"(b[r][1]), "=r"(b[r][2]), "=r"(b[r][3])
+                             : "r"(in_cta(at, (uint32_t)r)));
             else
                 asm volatile("ld.shared.v4.s32 {%0, %1, %2, %3}, [%4];"
-                             : "=r"(b[0]), "=r"(b[1]), "=r"(b[2]), "=r"(b[3]) : "r"(at));
-#pragma unroll
-            for (int j = 0; j < 4; ++j) a[j] += b[j];
+                             : "=r"(b[r][0]), "=r"(b[r][1]), "=r"(b[r][2]), "=r"(b[r][3]) : "r"(at));
         }
+#pragma unroll
+        for (int r = 0; r < S; ++r)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) a[j] += b[r][j];
         const float xsv = p.xs[m];
         const int64_t at_out = m * p.out_ld + n0 + c;
         float wsv[4], bv[4];
@@ -696,13 +757,19 @@ static int g_lin_configured[SS_MAX_DEVICES];
 static void *g_lin_ctx[SS_MAX_DEVICES];
 static int g_lin_nsm[SS_MAX_DEVICES];
 
+template <typename F>
+static cudaError_t linear_i8_split_attributes(F kernel) {
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)lin::split::MAX_SMEM);
+}
 template <int DT, bool GELU>
 static cudaError_t linear_i8_attributes() {
     cudaError_t e = cudaFuncSetAttribute(lin::pair::kernel<DT, GELU>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          (int)lin::pair::SMEM_BYTES);
-    if (e != cudaSuccess) return e;
-    return cudaFuncSetAttribute(lin::split::kernel<DT, GELU>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                (int)lin::split::MAX_SMEM);
+    if (e == cudaSuccess) e = linear_i8_split_attributes(lin::split::kernel<DT, GELU, 1>);
+    if (e == cudaSuccess) e = linear_i8_split_attributes(lin::split::kernel<DT, GELU, 2>);
+    if (e == cudaSuccess) e = linear_i8_split_attributes(lin::split::kernel<DT, GELU, 4>);
+    if (e == cudaSuccess) e = linear_i8_split_attributes(lin::split::kernel<DT, GELU, 8>);
+    return e;
 }
 
 int linear_i8_prepare(int device) {
@@ -789,7 +856,10 @@ static int launch(const Plan &plan, const int8_t *x, int64_t x_ld, const int8_t 
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return (int)cudaLaunchKernelEx(&cfg, split::kernel<DT, GELU>, tm_w, tm_x, p, plan.S);
+    if (plan.S == 1) return (int)cudaLaunchKernelEx(&cfg, split::kernel<DT, GELU, 1>, tm_w, tm_x, p);
+    if (plan.S == 2) return (int)cudaLaunchKernelEx(&cfg, split::kernel<DT, GELU, 2>, tm_w, tm_x, p);
+    if (plan.S == 4) return (int)cudaLaunchKernelEx(&cfg, split::kernel<DT, GELU, 4>, tm_w, tm_x, p);
+    return (int)cudaLaunchKernelEx(&cfg, split::kernel<DT, GELU, 8>, tm_w, tm_x, p);
 }
 
 }  // namespace lin
