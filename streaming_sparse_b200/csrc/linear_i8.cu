@@ -190,17 +190,17 @@ constexpr uint32_t W_BYTES = 128 * BK;           // 128 channels of a stage
 // epilogue warps of each CTA empty one tile while the next is summed.
 namespace pair {
 
-constexpr int EPI_WARPS = 8;
+constexpr int EPI_WARPS = 16;
 constexpr int THREADS = (EPI_WARPS + 2) * 32;
 constexpr uint32_t RING_BYTES = 6 * 2 * W_BYTES;               // six stages of the largest tile
 constexpr int MAX_STAGES = 10;
-constexpr uint32_t OFF_TURN = RING_BYTES;                      // per epilogue warp: 32 tokens x 32 channels of 16 bits
-constexpr uint32_t OFF_BAR = OFF_TURN + EPI_WARPS * 2048;
+constexpr uint32_t OFF_TURN = RING_BYTES;                      // per epilogue warp: 16 tokens x 32 channels of 16 bits
+constexpr uint32_t OFF_BAR = OFF_TURN + EPI_WARPS * 1024;
 enum Bar { FULL = 0, EMPTY = FULL + MAX_STAGES, ACC_FULL = EMPTY + MAX_STAGES, ACC_EMPTY = ACC_FULL + 2,
            DRAIN = ACC_EMPTY + 2, NBAR = DRAIN + 1 };
 constexpr uint32_t OFF_MISC = OFF_BAR + NBAR * 8 + (NBAR % 2) * 8;   // [0] tmem, [1] abort
 constexpr uint32_t OFF_XS = OFF_MISC + 16;
-constexpr uint32_t SMEM_BYTES = OFF_XS + EPI_WARPS * 128 * 4 + 1024;         // + alignment slack
+constexpr uint32_t SMEM_BYTES = OFF_XS + EPI_WARPS * 64 * 4 + 1024;         // + alignment slack
 
 __host__ __device__ constexpr uint32_t stage_bytes(int tn) { return W_BYTES + (uint32_t)(tn / 2) * BK; }
 // a smaller tile's stages are smaller, and its loop waits for the loads' latency: more of them fit
@@ -242,12 +242,12 @@ kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtenso
     const uint32_t tmem = misc[0];
 
     if (warp < EPI_WARPS) {
-        // ---------------- epilogue: 32 channels per warp, every other 32 tokens of the tile ----------------
+        // ---------------- epilogue: 32 channels per warp, every fourth 32 tokens of the tile ----------------
         const int wg = warp >> 2;
         const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
         const uint32_t acc_empty = in_cta(bar(ACC_EMPTY), 0);
-        float *xs_w = reinterpret_cast<float *>(smem + OFF_XS) + warp * 128;   // the tile's token scales
-        const uint32_t turn = sbase + OFF_TURN + (uint32_t)warp * 2048;
+        float *xs_w = reinterpret_cast<float *>(smem + OFF_XS) + warp * 64;   // the tile's token scales
+        const uint32_t turn = sbase + OFF_TURN + (uint32_t)warp * 1024;
         bool ok = true;
         int it = 0;
         for (int tile = pair_id; tile < p.ntiles && ok; tile += npairs, ++it) {
@@ -261,12 +261,12 @@ kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtenso
                 wsv[i] = n < p.N ? p.ws[n] : 0.f;
                 bv[i] = (p.bias && n < p.N) ? load_any(p.bias, p.bias_dtype, n) : 0.f;
             }
-            // the scales of the warp's tokens: 32-token chunks wg, wg + 2, ... of the tile
+            // the scales of the warp's tokens: 32-token chunks wg and wg + 4 of the tile
             __syncwarp();
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int64_t m = m0 + 32 * (2 * i + wg) + lane;
-                if (32 * (2 * i + wg) < p.tn) xs_w[32 * i + lane] = m < p.M ? p.xs[m] : 0.f;
+            for (int i = 0; i < 2; ++i) {
+                const int64_t m = m0 + 32 * (4 * i + wg) + lane;
+                if (32 * (4 * i + wg) < p.tn) xs_w[32 * i + lane] = m < p.M ? p.xs[m] : 0.f;
             }
             __syncwarp();
             const int b = it & 1;
@@ -274,28 +274,29 @@ kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtenso
             if (!ok) break;
             tc_fence_after();
             const uint32_t acc = lanes + 256 * b;
-            auto load = [&](int c, float (&v)[32]) {
+            for (int c = wg; c < p.tn / 32; c += 4) {
+                const int64_t mc = m0 + 32 * c;
+                const int rows = (int)min((int64_t)32, p.M - mc);
+                const float *xs_s = xs_w + 8 * (c - wg);
+                float v[32];
                 if (DT == SS_F32) {
                     tmem_ld32(acc + 32 * c, v);
                 } else {   // 16 channels x 32 tokens twice, as 8 x 8 fragments
                     tmem_ld_16x256b_x4(acc + 32 * c, v);
                     tmem_ld_16x256b_x4(acc + 32 * c + (16u << 16), v + 16);
                 }
-            };
-            auto store = [&](int c, float (&v)[32]) {
-                const int64_t mc = m0 + 32 * c;
-                const int rows = (int)min((int64_t)32, p.M - mc);
-                const float *xs_s = xs_w + 16 * (c - wg);
-                __syncwarp();   // the chunk before has left the warp's shared memory
+                tmem_wait_ld();
+                tmem_ld_fence32(v);
                 if constexpr (DT == SS_F32) {
-                    // thread = channel; half of the tokens at a time through shared memory, so that lane l
-                    // stores channels 4 (l % 8) .. + 4 of a token
+                    // thread = channel; 8 tokens at a time through shared memory, so that lane l stores
+                    // channels 4 (l % 8) .. + 4 of a token
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
+                    for (int h = 0; h < 4; ++h) {
+                        __syncwarp();   // the tokens before have left the warp's shared memory
 #pragma unroll
-                        for (int j = 0; j < 16; j += 2) {
-                            const float2 x2 = *reinterpret_cast<const float2 *>(xs_s + 16 * h + j);
-                            const uint64_t y = finish<GELU>(__float_as_int(v[16 * h + j]), __float_as_int(v[16 * h + j + 1]),
+                        for (int j = 0; j < 8; j += 2) {
+                            const float2 x2 = *reinterpret_cast<const float2 *>(xs_s + 8 * h + j);
+                            const uint64_t y = finish<GELU>(__float_as_int(v[8 * h + j]), __float_as_int(v[8 * h + j + 1]),
                                                             f2_mul(f2(x2.x, x2.y), f2(wsv[0], wsv[0])), f2(bv[0], bv[0]));
                             asm volatile("st.shared.f32 [%0], %1;" ::"r"(turn + 128u * j + 4u * lane), "f"(f2_lo(y)) : "memory");
                             asm volatile("st.shared.f32 [%0], %1;" ::"r"(turn + 128u * (j + 1) + 4u * lane), "f"(f2_hi(y)) : "memory");
@@ -303,8 +304,8 @@ kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtenso
                         __syncwarp();
                         const int nc = nw + 4 * (lane & 7);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int at = 4 * i + (lane >> 3), tok = 16 * h + at;
+                        for (int i = 0; i < 2; ++i) {
+                            const int at = 4 * i + (lane >> 3), tok = 8 * h + at;
                             float u[4];
                             asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
                                          : "=f"(u[0]), "=f"(u[1]), "=f"(u[2]), "=f"(u[3])
@@ -320,68 +321,56 @@ kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtenso
                                 }
                             }
                         }
-                        __syncwarp();
                     }
                 } else {
-                // v[16 h + 4 i + 2 e + t]: channel 16 h + 8 e + lane / 4, token 8 i + 2 (lane % 4) + t
+                    // v[16 h + 4 i + 2 e + t]: channel 16 h + 8 e + lane / 4, token 8 i + 2 (lane % 4) + t
+                    const int nc = nw + 8 * (lane & 3);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float2 x2 = *reinterpret_cast<const float2 *>(xs_s + 8 * i + 2 * (lane & 3));
-                    const uint64_t xs2 = f2(x2.x, x2.y);
-                    uint32_t o[4];
+                    for (int g = 0; g < 2; ++g) {   // 16 tokens at a time
+                        __syncwarp();   // the tokens before have left the warp's shared memory
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int at = 16 * (e >> 1) + 4 * i + 2 * (e & 1);
-                        const uint64_t y = finish<GELU>(__float_as_int(v[at]), __float_as_int(v[at + 1]),
-                                                        f2_mul(xs2, f2(wsv[e % NCH], wsv[e % NCH])),
-                                                        f2(bv[e % NCH], bv[e % NCH]));
-                        o[e] = pack2<DT>(f2_lo(y), f2_hi(y));
-                    }
-                    // transposed into rows of 32 channels: matrix e of the store is channels 8 e .. 8 e + 7 of
-                    // tokens 8 i .. 8 i + 7, lane l gives the row of token 8 i + l % 8 of matrix l / 8
-                    const int tok = 8 * i + (lane & 7);
-                    const uint32_t to = turn + (uint32_t)(tok * 64 + (((lane >> 3) ^ ((tok >> 1) & 3)) << 4));
-                    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};"
-                                 ::"r"(to), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]) : "memory");
-                }
-                __syncwarp();
-                // lane l: channels 8 (l % 4) .. + 8 of tokens l / 4 + 8 i
-                const int nc = nw + 8 * (lane & 3);
+                        for (int h = 0; h < 2; ++h) {
+                            const int i = 2 * g + h;
+                            const float2 x2 = *reinterpret_cast<const float2 *>(xs_s + 8 * i + 2 * (lane & 3));
+                            const uint64_t xs2 = f2(x2.x, x2.y);
+                            uint32_t o[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int tok = 8 * i + (lane >> 2);
-                    const uint32_t from = turn + (uint32_t)(tok * 64 + (((lane & 3) ^ ((tok >> 1) & 3)) << 4));
-                    uint4 u;
-                    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                                 : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "r"(from) : "memory");
-                    if (tok < rows) {
-                        uint16_t *dst = static_cast<uint16_t *>(p.out) + (mc + tok) * p.out_ld + nc;
-                        if (p.vec && nc + 7 < p.N) {
-                            *reinterpret_cast<uint4 *>(dst) = u;
-                        } else {
-                            const uint32_t w4[4] = {u.x, u.y, u.z, u.w};
+                            for (int e = 0; e < 4; ++e) {
+                                const int at = 16 * (e >> 1) + 4 * i + 2 * (e & 1);
+                                const uint64_t y = finish<GELU>(__float_as_int(v[at]), __float_as_int(v[at + 1]),
+                                                                f2_mul(xs2, f2(wsv[e % NCH], wsv[e % NCH])),
+                                                                f2(bv[e % NCH], bv[e % NCH]));
+                                o[e] = pack2<DT>(f2_lo(y), f2_hi(y));
+                            }
+                            // transposed into rows of 32 channels: matrix e of the store is channels 8 e .. 8 e + 7
+                            // of tokens 8 i .. 8 i + 7, lane l gives the row of token 8 i + l % 8 of matrix l / 8
+                            const int tok = 8 * h + (lane & 7);
+                            const uint32_t to = turn + (uint32_t)(tok * 64 + (((lane >> 3) ^ ((tok >> 1) & 3)) << 4));
+                            asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};"
+                                         ::"r"(to), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]) : "memory");
+                        }
+                        __syncwarp();
+                        // lane l: channels 8 (l % 4) .. + 8 of tokens l / 4 + 8 h
 #pragma unroll
-                            for (int j = 0; j < 8; ++j)
-                                if (nc + j < p.N) dst[j] = (uint16_t)(w4[j >> 1] >> (16 * (j & 1)));
+                        for (int h = 0; h < 2; ++h) {
+                            const int at = 8 * h + (lane >> 2), tok = 16 * g + at;
+                            const uint32_t from = turn + (uint32_t)(at * 64 + (((lane & 3) ^ ((at >> 1) & 3)) << 4));
+                            uint4 u;
+                            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                                         : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "r"(from) : "memory");
+                            if (tok < rows) {
+                                uint16_t *dst = static_cast<uint16_t *>(p.out) + (mc + tok) * p.out_ld + nc;
+                                if (p.vec && nc + 7 < p.N) {
+                                    *reinterpret_cast<uint4 *>(dst) = u;
+                                } else {
+                                    const uint32_t w4[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                                    for (int j = 0; j < 8; ++j)
+                                        if (nc + j < p.N) dst[j] = (uint16_t)(w4[j >> 1] >> (16 * (j & 1)));
+                                }
+                            }
                         }
                     }
-                }
-                }
-            };
-            // the next chunk comes out of TMEM while this one is finished and stored
-            const int nc = p.tn / 32;
-            float v0[32], v1[32];
-            if (wg < nc) load(wg, v0);
-            for (int c = wg; c < nc; c += 4) {
-                tmem_wait_ld();
-                tmem_ld_fence32(v0);
-                if (c + 2 < nc) load(c + 2, v1);
-                store(c, v0);
-                if (c + 2 < nc) {
-                    tmem_wait_ld();
-                    tmem_ld_fence32(v1);
-                    if (c + 4 < nc) load(c + 4, v0);
-                    store(c + 2, v1);
                 }
             }
             tc_fence_before();
@@ -801,24 +790,38 @@ struct Plan {
     int tn, S;
 };
 
+// Which kernel and tile, by a model of the time in us: a launch, then for each round of tiles the steps
+// over K and the tile's output. The constants are a fit to measured times (both kernels, every tile and
+// split, 5 to 4680 tokens x five weights of 1536 x 1536 to 8960 x 1536 and 1536 x 8960); the plan picked is
+// the fastest measured or within about 10 % of it. What it weighs, at 128 tokens (us): 1536 x 8960 weights, 11.0
+// split over clusters of 8 against 17.5 in pairs, whose steps follow one another; 4608 x 1536, 8.0 in pairs
+// against 8.8 in single CTAs, whose weights are read by twice the CTAs.
 static Plan choose(int M, int N, int K, int nsm) {
     const int npairs = nsm / 2;
     const int64_t ncb2 = (N + 255) / 256, ncb = (N + 127) / 128;
     const int nk = (K + BK - 1) / BK;
-    if (ncb2 * ((M + 255) / 256) * 2 >= npairs) {
-        Plan best = {true, 256, 1};
-        double cost = 1e30;
-        for (int tn = 256; tn >= 96; tn -= 32) {
-            const int64_t tiles = ncb2 * ((M + tn - 1) / tn);
-            const double c = (double)((tiles + npairs - 1) / npairs) * (tn + 64);
-            if (c < cost - 1e-9) cost = c, best.tn = tn;
-        }
-        return best;
+    Plan best = {true, 256, 1};
+    double least = 1e30;
+    for (int tn = 32; tn <= 256; tn += 32) {
+        if (tn > 32 && tn - 32 >= M) break;
+        const int64_t rounds = (ncb2 * ((M + tn - 1) / tn) + npairs - 1) / npairs;
+        // a step takes 0.18 us to hand on (0.2 with stores of earlier tiles under way); from 192 tokens its
+        // MMAs take longer
+        const double step = tn <= 160 ? (rounds > 1 ? 0.2 : 0.18) : 0.00108 * tn;
+        const double t = 4.5 + 0.01 * tn + (double)rounds * (nk * step + 0.2 + 0.004 * tn);
+        if (t < least) least = t, best = {true, tn, 1};
     }
-    Plan best = {false, 16, 1};
-    best.tn = M >= split::MAX_TN ? split::MAX_TN : (M + 15) / 16 * 16;
-    const int64_t tiles = ncb * ((M + best.tn - 1) / best.tn);
-    while (best.S < split::MAX_S && tiles * best.S * 2 <= nsm && best.S * 2 <= nk) best.S *= 2;
+    for (int tn = 16; tn <= split::MAX_TN; tn += 16) {
+        if (tn > 16 && tn - 16 >= M) break;
+        const int64_t tiles = ncb * ((M + tn - 1) / tn);
+        if (tiles > 2 * nsm) continue;
+        for (int S = 1; S <= split::MAX_S && S <= nk; S *= 2) {
+            const int64_t rounds = (tiles * S + nsm - 1) / nsm;
+            const double step = 0.2 + 0.0012 * tn;
+            const double t = 4.1 + (double)rounds * (step * ((nk + S - 1) / S) + 0.04 * tn) + 1.5 * (double)(rounds - 1);
+            if (t < least) least = t, best = {false, tn, S};
+        }
+    }
     return best;
 }
 
