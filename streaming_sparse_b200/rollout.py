@@ -174,7 +174,29 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.Tensor
 # ---------------------------------------------------------------------------------------------
 # model
 # ---------------------------------------------------------------------------------------------
+class Int8Linear:
+    """A linear layer on 8-bit rows: its weight as int8 with one scale for each output channel
+    (``ops.quant_rows``, once), applied to 8-bit activations by ``ops.linear_i8``."""
+
+    def __init__(self, lin: nn.Linear):
+        self.w = self.ws = None
+        self.load(lin)
+
+    def load(self, lin: nn.Linear) -> None:
+        """Quantise the layer's weight, into the buffers that captured graphs may already read."""
+        w = lin.weight.detach()
+        if self.w is not None and (self.w.shape, self.w.device) != (w.shape, w.device):
+            self.w = self.ws = None
+        self.w, self.ws = ops.quant_rows(w, out=self.w, scales=self.ws)
+        self.bias = lin.bias.detach()
+
+    def __call__(self, x_i8: torch.Tensor, xs: torch.Tensor, gelu: bool = False) -> torch.Tensor:
+        return ops.linear_i8(x_i8, xs, self.w, self.ws, bias=self.bias, gelu=gelu, out_dtype=self.bias.dtype)
+
+
 class Block(nn.Module):
+    INT8 = ("qkv", "o", "cq", "co", "ffn1", "ffn2")   # the layers that run per token
+
     def __init__(self, cfg: WanConfig):
         super().__init__()
         d = cfg.dim
@@ -194,6 +216,16 @@ class Block(nn.Module):
         self.ffn1 = nn.Linear(d, cfg.ffn_dim)
         self.ffn2 = nn.Linear(cfg.ffn_dim, d)
         self.modulation = nn.Parameter(torch.randn(1, 6, d) / d ** 0.5)
+        self._i8 = None
+
+    def quantize_linears(self) -> None:
+        """Lay the per-token linear layers' weights out in 8 bits, for ``forward(..., int8=True)``. Call it
+        again after the weights change; the bf16 weights stay."""
+        if self._i8 is None:
+            self._i8 = {name: Int8Linear(getattr(self, name)) for name in self.INT8}
+        else:
+            for name, lin in self._i8.items():
+                lin.load(getattr(self, name))
 
     def cross_kv(self, context: torch.Tensor):
         H = self.cfg.num_heads
@@ -201,14 +233,20 @@ class Block(nn.Module):
         v = self.cv(context).view(1, -1, H, HEAD_DIM)
         return k, v
 
-    def forward(self, x, e0, rope, cache: KVCache, cross, current_start: int, fused: bool = True):
+    def forward(self, x, e0, rope, cache: KVCache, cross, current_start: int, fused: bool = True,
+                int8: bool = False):
         """x [n, dim] bf16 (n = frames * frame_tokens), e0 [frames, 6, dim] fp32 -> new x.
 
         ``fused`` (CUDA only): the per-token work between the GEMMs runs in the library's
         kernels (AdaLN, q/k RMSNorm + RoPE with k/v written into the cache rows, RMSNorm, gated
         residual adds, in place on x); otherwise as the PyTorch expressions below, which state
-        the same arithmetic.
+        the same arithmetic. ``int8`` (fused, after ``quantize_linears``): the linear layers on 8-bit
+        rows, which the norms before them produce together with the residual adds.
         """
+        if int8:
+            if not (fused and x.is_cuda) or self._i8 is None:
+                raise ValueError("int8 needs the fused kernels on CUDA and quantize_linears()")
+            return self._forward_int8(x, e0, rope, cache, cross, current_start)
         if fused and x.is_cuda:
             return self._forward_fused(x, e0, rope, cache, cross, current_start)
         return self._forward_torch(x, e0, rope, cache, cross, current_start)
@@ -221,25 +259,7 @@ class Block(nn.Module):
         x = x.contiguous()
 
         h = ops.adaln(x, eps=cfg.eps, shift=em[:, 0], scale=em[:, 1], frame_tokens=ft)
-        qkv = self.qkv(h)
-        # a head-parallel rank's cache holds heads head0 .. head0 + cache.H - 1: q, k and v of
-        # those heads only (the q/k RMSNorm still over the whole width)
-        nh = cache.H
-        part = dict(model_heads=H, h0=cache.head0) if nh != H else {}
-        q = torch.empty((n, nh, HEAD_DIM), device=x.device, dtype=x.dtype)
-        rows = cache.reserve(n, current_start)
-        if rows is not None:
-            ops.qkv_norm_rope(qkv, self.norm_q, self.norm_k, cfg.eps, rope[0], rope[1], q, rows[0], rows[1], **part)
-        elif cache.ring_mode:   # straight into the ring rows, placed by the head in device memory
-            cache.write_qkv(qkv, self.norm_q, self.norm_k, cfg.eps, rope[0], rope[1], q, current_start,
-                            model_heads=H if part else None)
-        else:   # the write rolls the window: stage k/v, then the cache kernel rolls and writes
-            k = torch.empty_like(q)
-            v = torch.empty_like(q)
-            ops.qkv_norm_rope(qkv, self.norm_q, self.norm_k, cfg.eps, rope[0], rope[1], q, k, v, **part)
-            cache.append(k, v, current_start)
-        kw, vw = _window_for(cache)
-        y = _module_attention()(q[None], kw[None], vw[None])[0]
+        y = self._self_attention(self.qkv(h), rope, cache, current_start)
         ops.gate_residual(x, self.o(y.reshape(n, d)), gate=em[:, 2], frame_tokens=ft)
 
         hq = ops.rms_norm(self.cq(ops.adaln(x, eps=cfg.eps, weight=self.norm3_w, bias=self.norm3_b)), self.cnorm_q,
@@ -254,6 +274,54 @@ class Block(nn.Module):
         f1 = torch._addmm_activation(self.ffn1.bias, h, self.ffn1.weight.t(), use_gelu=True)
         ops.gate_residual(x, self.ffn2(f1), gate=em[:, 5], frame_tokens=ft)
         return x
+
+    def _forward_int8(self, x, e0, rope, cache: KVCache, cross, current_start: int):
+        """``_forward_fused`` with every per-token linear layer on 8-bit rows: each norm adds the
+        sublayer before it to the stream and writes the next one's 8-bit input."""
+        cfg, H, lin = self.cfg, self.cfg.num_heads, self._i8
+        n, d = x.shape
+        ft = n // e0.shape[0]
+        em = self.modulation.float() + e0                                 # [frames, 6, dim]
+        x = x.contiguous()
+
+        h = ops.adaln_i8(x, eps=cfg.eps, shift=em[:, 0], scale=em[:, 1], frame_tokens=ft)
+        y = self._self_attention(lin["qkv"](*h), rope, cache, current_start)
+        y = lin["o"](*ops.quant_rows(y.reshape(n, d)))
+
+        *h, x = ops.adaln_i8(x, eps=cfg.eps, weight=self.norm3_w, bias=self.norm3_b, y=y, gate=em[:, 2],
+                             frame_tokens=ft, sum_out=x)
+        hq = ops.rms_norm(lin["cq"](*h), self.cnorm_q, cfg.eps)
+        ck, cv = cross
+        y = dense_attention(hq.view(1, n, H, HEAD_DIM), ck, cv)[0]
+        y = lin["co"](*ops.quant_rows(y.reshape(n, d)))
+
+        *h, x = ops.adaln_i8(x, eps=cfg.eps, shift=em[:, 3], scale=em[:, 4], frame_tokens=ft, y=y, sum_out=x)
+        f1 = lin["ffn1"](*h, gelu=True)
+        ops.gate_residual(x, lin["ffn2"](*ops.quant_rows(f1)), gate=em[:, 5], frame_tokens=ft)
+        return x
+
+    def _self_attention(self, qkv, rope, cache: KVCache, current_start: int):
+        """The chunk's fused q/k/v [n, 3 dim] through q/k RMSNorm + RoPE and the cache into the attention."""
+        cfg, H = self.cfg, self.cfg.num_heads
+        n = qkv.shape[0]
+        # a head-parallel rank's cache holds heads head0 .. head0 + cache.H - 1: q, k and v of
+        # those heads only (the q/k RMSNorm still over the whole width)
+        nh = cache.H
+        part = dict(model_heads=H, h0=cache.head0) if nh != H else {}
+        q = torch.empty((n, nh, HEAD_DIM), device=qkv.device, dtype=qkv.dtype)
+        rows = cache.reserve(n, current_start)
+        if rows is not None:
+            ops.qkv_norm_rope(qkv, self.norm_q, self.norm_k, cfg.eps, rope[0], rope[1], q, rows[0], rows[1], **part)
+        elif cache.ring_mode:   # straight into the ring rows, placed by the head in device memory
+            cache.write_qkv(qkv, self.norm_q, self.norm_k, cfg.eps, rope[0], rope[1], q, current_start,
+                            model_heads=H if part else None)
+        else:   # the write rolls the window: stage k/v, then the cache kernel rolls and writes
+            k = torch.empty_like(q)
+            v = torch.empty_like(q)
+            ops.qkv_norm_rope(qkv, self.norm_q, self.norm_k, cfg.eps, rope[0], rope[1], q, k, v, **part)
+            cache.append(k, v, current_start)
+        kw, vw = _window_for(cache)
+        return _module_attention()(q[None], kw[None], vw[None])[0]
 
     def _forward_torch(self, x, e0, rope, cache: KVCache, cross, current_start: int):
         cfg, H = self.cfg, self.cfg.num_heads
@@ -371,16 +439,22 @@ class CausalWanDiT(nn.Module):
         u = torch.einsum("fhwpqrc->cfphqwr", u)
         return u.reshape(cfg.out_dim, Fr, cfg.latent_h, cfg.latent_w)
 
+    def quantize_linears(self) -> None:
+        """Lay out every block's per-token linear layers in 8 bits (``Block.quantize_linears``)."""
+        for blk in self.blocks:
+            blk.quantize_linears()
+
     def forward_chunk(self, x: torch.Tensor, t, caches, cross, start_frame: int, rope,
-                      fused: bool = True) -> torch.Tensor:
-        """x [C, F, Hl, Wl] latents of one chunk -> flow prediction [C, F, Hl, Wl]."""
+                      fused: bool = True, int8: bool = False) -> torch.Tensor:
+        """x [C, F, Hl, Wl] latents of one chunk -> flow prediction [C, F, Hl, Wl]; ``int8``: the
+        blocks' linear layers on 8-bit rows (``Block.forward``)."""
         cfg = self.cfg
         Fr = x.shape[1]
         e, e0 = self.embed_time(t, Fr, x.device)
         h = self.patchify(x)
         current_start = start_frame * cfg.frame_tokens
         for blk, cache, cr in zip(self.blocks, caches, cross):
-            h = blk(h, e0, rope, cache, cr, current_start, fused=fused)
+            h = blk(h, e0, rope, cache, cr, current_start, fused=fused, int8=int8)
         m = self.head_modulation.float() + e.unsqueeze(1)                     # [F, 2, dim]
         d = cfg.dim
         if fused and h.is_cuda:
@@ -403,6 +477,10 @@ class Rollout:
 
     ``fused`` selects the library's per-token kernels between the GEMMs (see ``Block.forward``).
 
+    ``int8_linears`` runs the blocks' linear layers on 8-bit rows (``ops.adaln_i8``, ``quant_rows``,
+    ``linear_i8``; one scale for each token and output channel); the weights are quantised here. The
+    text and time embeddings, the cross-attention's keys and values and the output head stay bf16.
+
     ``graphs=True``: the first ``run`` executes eagerly (it also warms up the libraries); from
     the second on, every model call (one chunk, one phase: 30 layers of GEMMs, norms, cache
     writes, routing and attention) is captured once into a CUDA graph and replayed, so the host
@@ -415,7 +493,7 @@ class Rollout:
     """
 
     def __init__(self, model: CausalWanDiT, sparse=None, scheduler: FlowMatch | None = None, graphs: bool = False,
-                 fused: bool = True, head_parallel: bool = False, group=None):
+                 fused: bool = True, head_parallel: bool = False, group=None, int8_linears: bool = False):
         self.model = model
         self.cfg = model.cfg
         self.sparse = sparse
@@ -445,6 +523,11 @@ class Rollout:
         self._rope = {}
         self.graphs = graphs
         self.fused = fused
+        self.int8_linears = int8_linears
+        if int8_linears:
+            if not fused:
+                raise ValueError("int8_linears runs with the fused kernels")
+            model.quantize_linears()
         self._runs = 0
         self._graph = {}          # (start_frame, frames, phase) -> (graph, x_in, t_in, flow_out)
         self._pool = None
@@ -517,7 +600,8 @@ class Rollout:
         """One model call on latents x [C, F, Hl, Wl] (any float dtype) -> flow prediction."""
         model = self.model
         if not use_graphs:
-            return model.forward_chunk(x.to(torch.bfloat16), t, self.caches, cross, c0, rope, fused=self.fused)
+            return model.forward_chunk(x.to(torch.bfloat16), t, self.caches, cross, c0, rope, fused=self.fused,
+                                       int8=self.int8_linears)
         # A call's device work is fixed by its shape, phase and the caches' index state (where
         # the chunk lands, whether the window rolls); the RoPE table comes through a static
         # buffer. So one graph serves every call with the same key -- with a rolling window, every
@@ -547,7 +631,8 @@ class Rollout:
                 self._pool = torch.cuda.graph_pool_handle()
             g = torch.cuda.CUDAGraph()
             with torch.cuda.graph(g, pool=self._pool):   # the host mirrors advance here, once
-                flow = model.forward_chunk(x_in, t_in, self.caches, cross, c0, rope_in, fused=self.fused)
+                flow = model.forward_chunk(x_in, t_in, self.caches, cross, c0, rope_in, fused=self.fused,
+                                           int8=self.int8_linears)
             ent = self._graph[key] = (g, x_in, t_in, flow)
             advance = False
         else:
@@ -619,6 +704,7 @@ def main(argv=None):
     ap.add_argument("--density", type=float, default=0.25)
     ap.add_argument("--dense", action="store_true", help="no plugin: dense attention everywhere")
     ap.add_argument("--unfused", action="store_true", help="PyTorch per-token ops instead of csrc/dit.cu")
+    ap.add_argument("--int8-linears", action="store_true", help="the blocks' linear layers on 8-bit rows")
     ap.add_argument("--layers", type=int, default=30)
     ap.add_argument("--frames", type=int, default=21)
     ap.add_argument("--runs", type=int, default=2)
@@ -643,7 +729,7 @@ def main(argv=None):
     if a.profile:
         from torch.profiler import ProfilerActivity, profile
 
-        ro = Rollout(model, sparse=sparse, fused=fused)
+        ro = Rollout(model, sparse=sparse, fused=fused, int8_linears=a.int8_linears)
         ro.run(noise, text, generator=g.manual_seed(2))
         c0 = cfg.frames - cfg.frames_per_chunk
         ctx = model.embed_text(text.bfloat16())
@@ -660,10 +746,10 @@ def main(argv=None):
                     if sparse is not None:
                         sparse.dense = phase == "clean"
                     t = 0.0 if phase == "clean" else ro.sched.denoising[1]
-                    model.forward_chunk(x, t, ro.caches, cross, c0, rope, fused=fused)
+                    model.forward_chunk(x, t, ro.caches, cross, c0, rope, fused=fused, int8=a.int8_linears)
                     torch.cuda.synchronize()
                     with profile(activities=[ProfilerActivity.CUDA]) as prof:
-                        model.forward_chunk(x, t, ro.caches, cross, c0, rope, fused=fused)
+                        model.forward_chunk(x, t, ro.caches, cross, c0, rope, fused=fused, int8=a.int8_linears)
                         torch.cuda.synchronize()
                     print(f"== {phase} call, chunk at frame {c0}, window {ro.caches[0].local_end} tokens")
                     print(prof.key_averages().table(sort_by="cuda_time_total", row_limit=16,
@@ -672,7 +758,7 @@ def main(argv=None):
             if plugin is not None:
                 plugin.__exit__(None, None, None)
         return
-    ro = Rollout(model, sparse=sparse, graphs=True, fused=fused)
+    ro = Rollout(model, sparse=sparse, graphs=True, fused=fused, int8_linears=a.int8_linears)
     for _ in range(2):
         ro.run(noise, text, generator=g.manual_seed(2))
     torch.cuda.synchronize()
