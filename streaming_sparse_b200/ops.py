@@ -907,13 +907,15 @@ def _rows_i8_in(x: torch.Tensor, name: str):
     return *x.shape, x.dtype, x.device
 
 
-def _rows_i8_out(out, scales, n: int, d: int, device):
-    if out is None:
-        out, ld = rows_i8(n, d, device), -(-d // 16) * 16
-    else:
+def _rows_i8_out(out, scales, x: torch.Tensor, n: int, d: int, device):
+    if out is not None:
         ld = _ld(out, "out", n, d, torch.int8, device)
+    elif d % 16 == 0:
+        out, ld = torch.empty_like(x, dtype=torch.int8, memory_format=torch.contiguous_format), d
+    else:
+        out, ld = rows_i8(n, d, device), -(-d // 16) * 16
     if scales is None:
-        scales = torch.empty(n, dtype=torch.float32, device=device)
+        scales = x.new_empty(n, dtype=torch.float32)
     else:
         _vec(scales, "scales", n, torch.float32, device)
     return out, ld, scales
@@ -929,7 +931,7 @@ def quant_rows(x: torch.Tensor, *, out: torch.Tensor | None = None, scales: torc
     n, d, dtype, dev = _rows_i8_in(x, "x")
     _no_grad(x)
     x_ld = _ld(x, "x", n, d, dtype, dev)
-    out, o_ld, scales = _rows_i8_out(out, scales, n, d, dev)
+    out, o_ld, scales = _rows_i8_out(out, scales, x, n, d, dev)
     rc = lib().ss_quant_rows(x.data_ptr(), x_ld, _I8_TYPES[dtype], n, d, out.data_ptr(), o_ld, scales.data_ptr(),
                              _stream_handle(dev))
     if rc:
@@ -966,7 +968,7 @@ def rms_norm_i8(x: torch.Tensor, weight: torch.Tensor, eps: float, *, residual: 
     x_ld = _ld(x, "x", n, d, dtype, dev)
     w = _vec(weight, "weight", d, dtype, dev)
     r, r_ld, s, sp, s_ld = _residual(residual, sum_out, "residual", n, d, dtype, dev)
-    out, o_ld, scales = _rows_i8_out(out, scales, n, d, dev)
+    out, o_ld, scales = _rows_i8_out(out, scales, x, n, d, dev)
     rc = lib().ss_rms_norm_i8(x.data_ptr(), x_ld, r, r_ld, _I8_TYPES[dtype], n, d, w, eps, sp, s_ld, out.data_ptr(),
                               o_ld, scales.data_ptr(), _stream_handle(dev))
     if rc:
@@ -1005,7 +1007,7 @@ def adaln_i8(x: torch.Tensor, *, eps: float, shift: torch.Tensor | None = None, 
             raise ValueError("gate goes with y")
         g_ld, gp = _frame_rows(gate, "gate", n, d, frame_tokens, dev), gate.data_ptr()
     r, r_ld, s, sp, s_ld = _residual(y, sum_out, "y", n, d, dtype, dev)
-    out, o_ld, scales = _rows_i8_out(out, scales, n, d, dev)
+    out, o_ld, scales = _rows_i8_out(out, scales, x, n, d, dev)
     rc = lib().ss_adaln_i8(x.data_ptr(), x_ld, r, r_ld, gp, g_ld, _I8_TYPES[dtype], n, d, frame_tokens, shp, scp,
                            mod_ld, wp, bp, eps, sp, s_ld, out.data_ptr(), o_ld, scales.data_ptr(),
                            _stream_handle(dev))
