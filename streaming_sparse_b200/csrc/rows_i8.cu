@@ -14,6 +14,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace ss {
@@ -120,13 +122,23 @@ struct Reduce {
     __device__ __forceinline__ uint32_t max_bits(uint32_t m) { return __float_as_uint((*this)(0.f, m).y); }
 };
 
+// Consecutive values a thread takes at a time. The LayerNorms take four: their fp32 vectors then come as
+// 16 bytes a lane without gaps. With eight (16 bytes of the 16-bit row) each lane's 32 bytes of a vector
+// come as two loads of every other 16 bytes, twice the passes through L1, which bounded the kernel
+// (32760 x 1536 AdaLN of bf16 45.6 us).
+template <typename T, int MODE, bool AL>
+__host__ __device__ constexpr int chunk_values() {
+    return AL && MODE < MOD ? 16 / (int)sizeof(T) : 4;
+}
+
 // VEC values of a row of d from c on, as loaded: 16 bytes at once (AL, d a multiple of VEC), or one by
 // one; zeros past the row's end (FULL: no chunk lies there)
 template <typename T, int VEC, bool AL, bool FULL>
 struct Chunk {
-    static constexpr int WORDS = (VEC * (int)sizeof(T) + 15) / 16;
+    static constexpr int BYTES = VEC * (int)sizeof(T), WORDS = BYTES <= 16 ? 1 : BYTES / 16;
+    using Word = typename std::conditional<BYTES == 8, uint2, uint4>::type;
     union {
-        uint4 u[WORDS];
+        Word u[WORDS];
         T e[VEC];
     };
     __device__ __forceinline__ Chunk() {}
@@ -134,7 +146,7 @@ struct Chunk {
         if constexpr (AL) {
 #pragma unroll
             for (int i = 0; i < WORDS; ++i)
-                u[i] = FULL || c < d ? reinterpret_cast<const uint4 *>(src + c)[i] : make_uint4(0u, 0u, 0u, 0u);
+                u[i] = FULL || c < d ? reinterpret_cast<const Word *>(src + c)[i] : Word{};
         } else {
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
@@ -148,7 +160,7 @@ struct Chunk {
         if constexpr (AL) {
 #pragma unroll
             for (int i = 0; i < WORDS; ++i)
-                if (FULL || c < d) reinterpret_cast<uint4 *>(dst + c)[i] = u[i];
+                if (FULL || c < d) reinterpret_cast<Word *>(dst + c)[i] = u[i];
         } else {
 #pragma unroll
             for (int j = 0; j < VEC; ++j)
@@ -196,7 +208,7 @@ __device__ __forceinline__ void store_codes(int8_t *out, int c, int d, int words
 template <typename T, int MODE, bool WARP, int NE, bool AL, bool FULL>
 __global__ void __launch_bounds__(WARP || NE == 16 ? 128 : NE == 24 ? 1024 : NE == 40 ? 256 : 512,
                                   NE == 48 && MODE == QUANT && !WARP ? 2 : 0) row_kernel(const Args p) {
-    constexpr int VEC = AL ? 16 / (int)sizeof(T) : 4, NV = NE / VEC;
+    constexpr int VEC = chunk_values<T, MODE, AL>(), NV = NE / VEC;
     __shared__ float2 red[2][32];
     Reduce<WARP> reduce{red};
     const int t = WARP ? (int)(threadIdx.x & 31) : (int)threadIdx.x, G = WARP ? 32 : (int)blockDim.x, d = p.d;
@@ -386,7 +398,7 @@ static void launch_warps(const Args &p, cudaStream_t st) {
 }
 template <typename T, int MODE, int NE, bool AL>
 static void launch_blocks(const Args &p, cudaStream_t st) {
-    constexpr int VEC = AL ? 16 / (int)sizeof(T) : 4, NV = NE / VEC;
+    constexpr int VEC = chunk_values<T, MODE, AL>(), NV = NE / VEC;
     const int chunks = (p.d + VEC - 1) / VEC, threads = ((chunks + NV - 1) / NV + 31) / 32 * 32;
     if (AL && p.d == threads * NE) row_kernel<T, MODE, false, NE, AL, AL><<<p.n, threads, 0, st>>>(p);
     else row_kernel<T, MODE, false, NE, AL, false><<<p.n, threads, 0, st>>>(p);
@@ -405,11 +417,12 @@ static int launch_rows(const Args &p, cudaStream_t st) {
 
 template <typename T, int MODE>
 static int launch_type(Args p, cudaStream_t st) {
-    constexpr int VEC = 16 / (int)sizeof(T);
-    // rows and vectors all start at 16-byte boundaries and end at a whole vector
-    const bool al = p.d % VEC == 0 && !off(p.x, 16) && p.x_ld % VEC == 0 && !off(p.weight, 16) && !off(p.bias, 16) &&
-                    (!p.res || (!off(p.res, 16) && p.res_ld % VEC == 0)) &&
-                    (!p.sum || (!off(p.sum, 16) && p.sum_ld % VEC == 0)) &&
+    constexpr int VEC = chunk_values<T, MODE, true>();
+    constexpr size_t bytes = VEC * sizeof(T);
+    // rows and vectors all start at a chunk's boundary and end at a whole chunk
+    const bool al = p.d % VEC == 0 && !off(p.x, bytes) && p.x_ld % VEC == 0 && !off(p.weight, bytes) &&
+                    !off(p.bias, bytes) && (!p.res || (!off(p.res, bytes) && p.res_ld % VEC == 0)) &&
+                    (!p.sum || (!off(p.sum, bytes) && p.sum_ld % VEC == 0)) &&
                     (!p.gate || (!off(p.gate, 16) && p.gate_ld % 4 == 0)) &&
                     (!p.shift || (!off(p.shift, 16) && !off(p.scale, 16) && p.mod_ld % 4 == 0));
     p.inv_d = 1.f / (float)p.d;
