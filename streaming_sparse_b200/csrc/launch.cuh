@@ -1,0 +1,35 @@
+// launch.cuh -- programmatic dependent launch for kernels that follow one another on a stream.
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include <utility>
+
+namespace ss {
+
+// Waits until the grids before this one on the stream are complete and their memory is visible. Every
+// thread of a kernel started by launch_after() calls it before it touches global memory.
+__device__ __forceinline__ void wait_for_earlier() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// Lets the next such kernel on the stream set itself up once every block of this one has got here.
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+template <typename K, typename... A>
+static cudaError_t launch_after(K kernel, unsigned blocks, unsigned threads, size_t smem, cudaStream_t st, unsigned cluster,
+                                const A &...args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(blocks);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+}  // namespace ss

@@ -11,6 +11,7 @@
 #include <mutex>
 
 #include "common.cuh"
+#include "launch.cuh"
 
 namespace ss {
 
@@ -239,6 +240,8 @@ kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtenso
     __syncthreads();
     cluster_sync();   // both CTAs' barriers are initialised before either is signalled from the other
     tc_fence_after();
+    let_next_start();
+    wait_for_earlier();
     const uint32_t tmem = misc[0];
 
     if (warp < EPI_WARPS) {
@@ -515,6 +518,8 @@ kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtenso
     }
     __syncthreads();
     tc_fence_after();
+    let_next_start();
+    wait_for_earlier();
     const uint32_t tmem = misc[0];
     int *sums = reinterpret_cast<int *>(smem);   // [tn][128], over the stages once they are consumed
     bool ok = true;
@@ -661,6 +666,8 @@ template <int DT, bool GELU, int MT, int CH, int WPC>
 __global__ void __launch_bounds__(WARPS * 32)
 kernel(const int8_t *__restrict__ x, int64_t x_ld, const int8_t *__restrict__ w, int64_t w_ld, const Params p) {
     __shared__ int red[WARPS][CH * MT];
+    let_next_start();
+    wait_for_earlier();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % WPC;
     const int n0 = (blockIdx.x * (WARPS / WPC) + warp / WPC) * CH;
     const int chunks = (p.K + 15) / 16;
@@ -726,11 +733,10 @@ static int launch(const int8_t *x, int64_t x_ld, const int8_t *w, int64_t w_ld, 
     int wpc = 1;
     while (wpc < WARPS && groups * wpc < 16 * (int64_t)nsm && wpc * 2 <= steps) wpc *= 2;
     const unsigned blocks = (unsigned)((groups * wpc + WARPS - 1) / WARPS);
-    if (wpc == 1) kernel<DT, GELU, MT, CH, 1><<<blocks, WARPS * 32, 0, st>>>(x, x_ld, w, w_ld, p);
-    else if (wpc == 2) kernel<DT, GELU, MT, CH, 2><<<blocks, WARPS * 32, 0, st>>>(x, x_ld, w, w_ld, p);
-    else if (wpc == 4) kernel<DT, GELU, MT, CH, 4><<<blocks, WARPS * 32, 0, st>>>(x, x_ld, w, w_ld, p);
-    else kernel<DT, GELU, MT, CH, 8><<<blocks, WARPS * 32, 0, st>>>(x, x_ld, w, w_ld, p);
-    return (int)cudaGetLastError();
+    if (wpc == 1) return (int)launch_after(kernel<DT, GELU, MT, CH, 1>, blocks, WARPS * 32, 0, st, 1, x, x_ld, w, w_ld, p);
+    if (wpc == 2) return (int)launch_after(kernel<DT, GELU, MT, CH, 2>, blocks, WARPS * 32, 0, st, 1, x, x_ld, w, w_ld, p);
+    if (wpc == 4) return (int)launch_after(kernel<DT, GELU, MT, CH, 4>, blocks, WARPS * 32, 0, st, 1, x, x_ld, w, w_ld, p);
+    return (int)launch_after(kernel<DT, GELU, MT, CH, 8>, blocks, WARPS * 32, 0, st, 1, x, x_ld, w, w_ld, p);
 }
 
 }  // namespace dot
@@ -844,25 +850,19 @@ static int launch(const Plan &plan, const int8_t *x, int64_t x_ld, const int8_t 
         if (tiles > 0x7fffffff) return SS_ERR_SHAPE;
         p.ntiles = (int)tiles;
         const int npairs = (int)(tiles < nsm / 2 ? tiles : nsm / 2);
-        pair::kernel<DT, GELU><<<2 * npairs, pair::THREADS, pair::SMEM_BYTES, st>>>(tm_w, tm_x, p);
-        return (int)cudaGetLastError();
+        return (int)launch_after(pair::kernel<DT, GELU>, 2u * (unsigned)npairs, pair::THREADS, pair::SMEM_BYTES, st, 1, tm_w,
+                                 tm_x, p);
     }
     p.ncb = (p.N + 127) / 128;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(p.ncb * ntb * plan.S));
-    cfg.blockDim = dim3(split::THREADS);
-    cfg.dynamicSmemBytes = split::smem_bytes(plan.tn);
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)plan.S;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    if (plan.S == 1) return (int)cudaLaunchKernelEx(&cfg, split::kernel<DT, GELU, 1>, tm_w, tm_x, p);
-    if (plan.S == 2) return (int)cudaLaunchKernelEx(&cfg, split::kernel<DT, GELU, 2>, tm_w, tm_x, p);
-    if (plan.S == 4) return (int)cudaLaunchKernelEx(&cfg, split::kernel<DT, GELU, 4>, tm_w, tm_x, p);
-    return (int)cudaLaunchKernelEx(&cfg, split::kernel<DT, GELU, 8>, tm_w, tm_x, p);
+    const unsigned blocks = (unsigned)(p.ncb * ntb * plan.S);
+    const size_t smem = split::smem_bytes(plan.tn);
+    auto go = [&](auto kernel) {
+        return (int)launch_after(kernel, blocks, split::THREADS, smem, st, (unsigned)plan.S, tm_w, tm_x, p);
+    };
+    if (plan.S == 1) return go(split::kernel<DT, GELU, 1>);
+    if (plan.S == 2) return go(split::kernel<DT, GELU, 2>);
+    if (plan.S == 4) return go(split::kernel<DT, GELU, 4>);
+    return go(split::kernel<DT, GELU, 8>);
 }
 
 }  // namespace lin

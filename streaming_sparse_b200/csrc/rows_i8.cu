@@ -17,6 +17,7 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "launch.cuh"
 
 namespace ss {
 namespace rows {
@@ -210,6 +211,8 @@ __global__ void __launch_bounds__(WARP || NE == 16 ? 128 : NE == 24 ? 1024 : NE 
                                   NE == 48 && MODE == QUANT && !WARP ? 2 : 0) row_kernel(const Args p) {
     constexpr int VEC = chunk_values<T, MODE, AL>(), NV = NE / VEC;
     __shared__ float2 red[2][32];
+    let_next_start();
+    wait_for_earlier();
     Reduce<WARP> reduce{red};
     const int t = WARP ? (int)(threadIdx.x & 31) : (int)threadIdx.x, G = WARP ? 32 : (int)blockDim.x, d = p.d;
     const int64_t row = WARP ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5) : (int64_t)blockIdx.x;
@@ -333,6 +336,8 @@ __global__ void __launch_bounds__(WARP || NE == 16 ? 128 : NE == 24 ? 1024 : NE 
 template <typename T, int MODE>
 __global__ void __launch_bounds__(512) long_row_kernel(const Args p) {
     __shared__ float2 red[2][32];
+    let_next_start();
+    wait_for_earlier();
     Reduce<false> reduce{red};
     const int64_t row = blockIdx.x;
     const int t = threadIdx.x, d = p.d;
@@ -393,15 +398,15 @@ static bool off(const void *p, size_t a) { return (reinterpret_cast<uintptr_t>(p
 template <typename T, int MODE, int NE, bool AL>
 static void launch_warps(const Args &p, cudaStream_t st) {
     const unsigned blocks = (unsigned)(((int64_t)p.n + 3) / 4);
-    if (AL && p.d == 32 * NE) row_kernel<T, MODE, true, NE, AL, AL><<<blocks, 128, 0, st>>>(p);
-    else row_kernel<T, MODE, true, NE, AL, false><<<blocks, 128, 0, st>>>(p);
+    if (AL && p.d == 32 * NE) launch_after(row_kernel<T, MODE, true, NE, AL, AL>, blocks, 128, 0, st, 1, p);
+    else launch_after(row_kernel<T, MODE, true, NE, AL, false>, blocks, 128, 0, st, 1, p);
 }
 template <typename T, int MODE, int NE, bool AL>
 static void launch_blocks(const Args &p, cudaStream_t st) {
     constexpr int VEC = chunk_values<T, MODE, AL>(), NV = NE / VEC;
     const int chunks = (p.d + VEC - 1) / VEC, threads = ((chunks + NV - 1) / NV + 31) / 32 * 32;
-    if (AL && p.d == threads * NE) row_kernel<T, MODE, false, NE, AL, AL><<<p.n, threads, 0, st>>>(p);
-    else row_kernel<T, MODE, false, NE, AL, false><<<p.n, threads, 0, st>>>(p);
+    if (AL && p.d == threads * NE) launch_after(row_kernel<T, MODE, false, NE, AL, AL>, p.n, threads, 0, st, 1, p);
+    else launch_after(row_kernel<T, MODE, false, NE, AL, false>, p.n, threads, 0, st, 1, p);
 }
 template <typename T, int MODE, bool AL>
 static int launch_rows(const Args &p, cudaStream_t st) {
@@ -411,7 +416,7 @@ static int launch_rows(const Args &p, cudaStream_t st) {
     else if (p.d <= 128 * 16) launch_blocks<T, MODE, 16, AL>(p, st);
     else if (p.d <= 256 * 40) launch_blocks<T, MODE, 40, AL>(p, st);
     else if (p.d <= 512 * 48) launch_blocks<T, MODE, sizeof(T) == 4 ? 24 : 48, AL>(p, st);   // registers
-    else long_row_kernel<T, MODE><<<p.n, 512, 0, st>>>(p);
+    else launch_after(long_row_kernel<T, MODE>, p.n, 512, 0, st, 1, p);
     return (int)cudaGetLastError();
 }
 
