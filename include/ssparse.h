@@ -529,7 +529,8 @@ int ss_gate_residual(void *x, const void *y, int64_t y_ld, int n, int d, int fra
 /* least 1e-30, so a row of zeros has finite codes). A row that holds an infinity or a NaN gets  */
 /* codes 0 and scale NaN: its products are NaN, and no other row's are. Rows of every buffer may */
 /* lie at any stride (in elements, at least d); `dtype` is SS_BF16, SS_F32 or SS_F16 and holds   */
-/* for x, the residual, the norm's weight and bias, and the stored sum. n may be 0.              */
+/* for x, the residual, the norm's weight and bias, and the stored sum. n may be 0. The kernels    */
+/* start while the one before them on the stream ends, and wait for it before they touch memory.  */
 /* ------------------------------------------------------------------------------------------ */
 
 /* q = rint(x * (1 / s)) for rows x [n][d] -> out [n][d] int8, scales [n]. */
@@ -562,7 +563,8 @@ int ss_adaln_i8(const void *x, int64_t x_ld, const void *y, int64_t y_ld, const 
 
 /* out[m][n] = act(S * (xs[m] * ws[n]) + bias[n]), S = sum_k x[m][k] * w[n][k] exact in 32 bits; act
  * is the tanh form of GELU where gelu != 0, else the identity. x [M][K] and w [N][K] int8, 16-byte
- * aligned with row strides that are multiples of 16; bias [N] of bias_dtype or NULL; out [M][N] of
+ * aligned with row strides that are multiples of 16 (a row's last 16 bytes may be read whole; what lies
+ * past K counts for nothing); bias [N] of bias_dtype or NULL; out [M][N] of
  * out_dtype, row stride out_ld. `status` (optional) gets SS_DEV_TIMEOUT if a wait in the kernel ran
  * out. M may be 0. */
 int ss_linear_i8(const int8_t *x, int64_t x_ld, const float *xs, const int8_t *w, int64_t w_ld,
