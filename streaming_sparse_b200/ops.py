@@ -1045,7 +1045,7 @@ def linear_i8(x_i8: torch.Tensor, xs: torch.Tensor, w_i8: torch.Tensor, ws: torc
     if out is None:
         if out_dtype not in _I8_TYPES:
             raise ValueError("out_dtype: bfloat16, float16 or float32 expected")
-        out, o_ld = torch.empty((M, N), dtype=out_dtype, device=dev), N
+        out, o_ld = xs.new_empty((M, N), dtype=out_dtype), N
     else:
         out_dtype = out.dtype
         if out_dtype not in _I8_TYPES:
