@@ -8,7 +8,9 @@
 namespace ss {
 
 // Waits until the grids before this one on the stream are complete and their memory is visible. Every
-// thread of a kernel started by launch_after() calls it before it touches global memory.
+// thread of a kernel started by launch_after() calls it before it touches global memory, and such a
+// kernel reads nothing through the non-coherent path (ld.global.nc, const __restrict__): its inputs may
+// still be written while it already runs.
 __device__ __forceinline__ void wait_for_earlier() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 // Lets the next such kernel on the stream set itself up once every block of this one has got here.
 __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }

@@ -684,7 +684,7 @@ constexpr int WARPS = 8;
 
 template <int DT, bool GELU, int MT, int CH, int WPC>
 __global__ void __launch_bounds__(WARPS * 32)
-kernel(const int8_t *__restrict__ x, int64_t x_ld, const int8_t *__restrict__ w, int64_t w_ld, const Params p) {
+kernel(const int8_t *x, int64_t x_ld, const int8_t *w, int64_t w_ld, const Params p) {
     __shared__ int red[WARPS][CH * MT];
     let_next_start();
     wait_for_earlier();
@@ -700,7 +700,8 @@ kernel(const int8_t *__restrict__ x, int64_t x_ld, const int8_t *__restrict__ w,
         uint4 a[CH];
 #pragma unroll
         for (int c = 0; c < CH; ++c)
-            asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+            // not .nc: this kernel may have started before the one that wrote its inputs ended
+            asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
                          : "=r"(a[c].x), "=r"(a[c].y), "=r"(a[c].z), "=r"(a[c].w) : "l"(wr[c] + k));
         const int left = p.K - 16 * k;   // codes of this chunk that are the row's
 #pragma unroll
@@ -892,8 +893,9 @@ extern "C" int ss_linear_i8(const int8_t *x, int64_t x_ld, const float *xs, cons
                             const float *ws, const void *bias, int bias_dtype, int gelu, int M, int N, int K,
                             void *out, int64_t out_ld, int out_dtype, int *status, void *stream) {
     using namespace ss;
-    if (M < 0 || N <= 0 || K <= 0 || K > SS_LINEAR_I8_MAX_K || M > SS_LINEAR_I8_MAX_ROWS || N > SS_LINEAR_I8_MAX_ROWS || x_ld < K || w_ld < K || out_ld < N || (x_ld % 16) ||
-        (w_ld % 16) || !lin::known(out_dtype) || (bias && !lin::known(bias_dtype)))
+    if (M < 0 || N <= 0 || K <= 0 || K > SS_LINEAR_I8_MAX_K || M > SS_LINEAR_I8_MAX_ROWS ||
+        N > SS_LINEAR_I8_MAX_ROWS || x_ld < K || w_ld < K || out_ld < N || (x_ld % 16) || (w_ld % 16) ||
+        !lin::known(out_dtype) || (bias && !lin::known(bias_dtype)))
         return SS_ERR_SHAPE;
     if (M == 0) return 0;   // buffers without rows may have no address
     if (!x || !xs || !w || !ws || !out) return SS_ERR_POINTER;
