@@ -53,6 +53,12 @@ int encode_tmap_2d_bf16_rows(CUtensorMap *map, const void *base, uint64_t inner,
     return encode_2d_bf16(map, base, inner, outer, row_stride_bytes, box_inner, box_outer, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
+// 2-D tensor map of 16-bit values with 64-byte swizzle, for stores of boxes 32 values wide.
+int encode_tmap_2d_b16_sw64(CUtensorMap *map, const void *base, uint64_t inner, uint64_t outer,
+                            uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_outer) {
+    return encode_2d_bf16(map, base, inner, outer, row_stride_bytes, box_inner, box_outer, CU_TENSOR_MAP_SWIZZLE_64B);
+}
+
 // 2-D uint8 tensor map over a row-major [outer][inner] view (int8 data), 128-byte swizzle.
 int encode_tmap_2d_u8(CUtensorMap *map, const void *base, uint64_t inner, uint64_t outer, uint64_t row_stride_bytes,
                       uint32_t box_inner, uint32_t box_outer) {

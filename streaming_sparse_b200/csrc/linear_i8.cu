@@ -10,8 +10,8 @@
 // tokens (latency), SM pairs for many (L2 and the tensor pipe). Measured on B200 (buffers beyond L2):
 //   one token x 8960 x 1536, GELU          4.1 us, 3.4 TB/s of weights (2.9 us from L2)
 //   77 x 1531 x 1549 to fp32               6.7 us
-//   4680 x 4608 x 1536                    27.9 us, 2.38 POPS
-//   4680 x 8960 x 1536, GELU              56.3 us, 2.29 POPS (51.0 us without GELU)
+//   4680 x 4608 x 1536                    27.7 us, 2.39 POPS
+//   4680 x 8960 x 1536, GELU              54.9 us, 2.35 POPS (50.7 us without GELU)
 //   4680 x 1536 x 8960 to fp16            44.3 us, 2.91 POPS
 //   32760 x 8960 x 1536, GELU              380 us, 2.37 POPS (power-limited)
 // The library's 8-bit product of these sizes, which stops at the 32-bit sums: 29.7, 54.0, 48.2, 352 us.
@@ -27,6 +27,8 @@ namespace ss {
 
 int encode_tmap_2d_u8(CUtensorMap *map, const void *base, uint64_t inner, uint64_t outer, uint64_t row_stride_bytes,
                       uint32_t box_inner, uint32_t box_outer);
+int encode_tmap_2d_b16_sw64(CUtensorMap *map, const void *base, uint64_t inner, uint64_t outer,
+                            uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_outer);
 
 namespace lin {
 
@@ -41,7 +43,7 @@ struct Params {
     int tn;      // tokens a tile
     int ncb;     // channel blocks
     int ntiles;  // channel blocks x token blocks (pairs)
-    int vec;     // rows of out take 16-byte stores (pairs), 4-channel stores (split)
+    int vec;     // rows of out start at 16 bytes (pairs: TMA or 16-byte stores), 4 channels (split)
 };
 
 __device__ __forceinline__ float load_any(const void *p, int dtype, int64_t i) {
@@ -103,6 +105,18 @@ __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap
         " [%0], [%1, {%2, %3}], [%4];"
         ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
         : "memory");
+}
+// a box of this CTA's shared memory to the tensor at {x, y}, clipped to the tensor
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap *map, int x, int y, uint32_t src) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];"
+                 ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(src)
+                 : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+// until all but the latest LEFT of this thread's bulk groups have read their shared memory
+template <int LEFT>
+__device__ __forceinline__ void bulk_read_wait() {
+    asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(LEFT) : "memory");
 }
 // D[tmem] (+)= A[smem] * B[smem], kind::i8 (s8 inputs, s32 accumulate)
 template <int CTAS>
@@ -204,27 +218,30 @@ constexpr uint32_t W_BYTES = 128 * BK;           // 128 channels of a stage
 // already delivers 17 TB/s at 256 x 256 (0.277 us a step, 0.27 at the tensor pipe's rate). What
 // bounds it, by leaving parts out: 4680 x 8960 x 1536 takes 51.0 us, 39.9 without the stores of the 84 MB of
 // outputs, 38.0 without the epilogue: the stores, which share L2 with the loads. Eight epilogue warps were
-// latency bound at two a scheduler (54.4 us, 64 with GELU against 56.3).
+// latency bound at two a scheduler (54.4 us, 64 with GELU against 56.3). 16-bit outputs leave as TMA boxes of
+// 16 tokens x 32 channels; stored by the warps themselves they took 51.5 us (57 with GELU against 54.9).
 namespace pair {
 
 constexpr int EPI_WARPS = 16;
 constexpr int THREADS = (EPI_WARPS + 2) * 32;
 constexpr uint32_t RING_BYTES = 6 * 2 * W_BYTES;               // six stages of the largest tile
 constexpr int MAX_STAGES = 10;
-constexpr uint32_t OFF_TURN = RING_BYTES;                      // per epilogue warp: 16 tokens x 32 channels of 16 bits
-constexpr uint32_t OFF_BAR = OFF_TURN + EPI_WARPS * 1024;
+// per epilogue warp 2 KB: two halves of 16 tokens x 32 channels of 16 bits; or, for 32-bit outputs,
+// 8 tokens x 32 channels and the token scales
+constexpr uint32_t OFF_TURN = RING_BYTES;
+constexpr uint32_t OFF_BAR = OFF_TURN + EPI_WARPS * 2048;
 enum Bar { FULL = 0, EMPTY = FULL + MAX_STAGES, ACC_FULL = EMPTY + MAX_STAGES, ACC_EMPTY = ACC_FULL + 2,
            DRAIN = ACC_EMPTY + 2, NBAR = DRAIN + 1 };
 constexpr uint32_t OFF_MISC = OFF_BAR + NBAR * 8 + (NBAR % 2) * 8;   // [0] tmem, [1] abort
-constexpr uint32_t OFF_XS = OFF_MISC + 16;
-constexpr uint32_t SMEM_BYTES = OFF_XS + EPI_WARPS * 64 * 4 + 1024;         // + alignment slack
+constexpr uint32_t SMEM_BYTES = OFF_MISC + 16 + 1024;                // + alignment slack
 
 __host__ __device__ constexpr uint32_t stage_bytes(int tn) { return W_BYTES + (uint32_t)(tn / 2) * BK; }
 // a smaller tile's stages are smaller, and its loop waits for the loads' latency: more of them fit
 
 template <int DT, bool GELU>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
-kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, const Params p) {
+kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
+       const __grid_constant__ CUtensorMap tm_out, const Params p) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const uint32_t sbase = smem_u32(smem);
@@ -246,6 +263,7 @@ kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtenso
         *abort_flag = 0;
         prefetch_tmap(&tm_w);
         prefetch_tmap(&tm_x);
+        if (DT != SS_F32 && p.vec) prefetch_tmap(&tm_out);
     }
     if (warp == 0) {
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(sbase + OFF_MISC),
@@ -265,8 +283,8 @@ kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtenso
         const int wg = warp >> 2;
         const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
         const uint32_t acc_empty = in_cta(bar(ACC_EMPTY), 0);
-        float *xs_w = reinterpret_cast<float *>(smem + OFF_XS) + warp * 64;   // the tile's token scales
-        const uint32_t turn = sbase + OFF_TURN + (uint32_t)warp * 1024;
+        const uint32_t turn = sbase + OFF_TURN + (uint32_t)warp * 2048;
+        float *xs_w = reinterpret_cast<float *>(smem + OFF_TURN + warp * 2048 + 1024);   // 32-bit outputs: token scales
         bool ok = true;
         int it = 0;
         for (int tile = pair_id; tile < p.ntiles && ok; tile += npairs, ++it) {
@@ -280,23 +298,37 @@ kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtenso
                 wsv[i] = n < p.N ? p.ws[n] : 0.f;
                 bv[i] = (p.bias && n < p.N) ? load_any(p.bias, p.bias_dtype, n) : 0.f;
             }
-            // the scales of the warp's tokens: 32-token chunks wg and wg + 4 of the tile
-            __syncwarp();
+            // the scales of the warp's tokens, 32-token chunks wg and wg + 4 of the tile: all of them in shared
+            // memory, or this thread's tokens 8 i + 2 (lane % 4) + {0, 1} of each
+            uint64_t xsv[2][4];
+            if (DT == SS_F32) {
+                __syncwarp();
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int64_t m = m0 + 32 * (4 * i + wg) + lane;
-                if (32 * (4 * i + wg) < p.tn) xs_w[32 * i + lane] = m < p.M ? p.xs[m] : 0.f;
+                for (int i = 0; i < 2; ++i) {
+                    const int64_t m = m0 + 32 * (4 * i + wg) + lane;
+                    if (32 * (4 * i + wg) < p.tn) xs_w[32 * i + lane] = m < p.M ? p.xs[m] : 0.f;
+                }
+                __syncwarp();
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int64_t m = m0 + 32 * (4 * (i >> 2) + wg) + 8 * (i & 3) + 2 * (lane & 3);
+                    const bool in = 32 * (4 * (i >> 2) + wg) < p.tn;
+                    xsv[i >> 2][i & 3] = f2(in && m < p.M ? p.xs[m] : 0.f, in && m + 1 < p.M ? p.xs[m + 1] : 0.f);
+                }
             }
-            __syncwarp();
             const int b = it & 1;
             ok = warp_all(mbar_wait(bar(ACC_FULL + b), (it >> 1) & 1, abort_flag));
             if (!ok) break;
             tc_fence_after();
             const uint32_t acc = lanes + 256 * b;
-            for (int c = wg; c < p.tn / 32; c += 4) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int c = wg + 4 * u;
+                if (c >= p.tn / 32) break;
                 const int64_t mc = m0 + 32 * c;
                 const int rows = (int)min((int64_t)32, p.M - mc);
-                const float *xs_s = xs_w + 8 * (c - wg);
+                const float *xs_s = xs_w + 32 * u;
                 float v[32];
                 if (DT == SS_F32) {
                     tmem_ld32(acc + 32 * c, v);
@@ -345,48 +377,50 @@ kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtenso
                     // v[16 h + 4 i + 2 e + t]: channel 16 h + 8 e + lane / 4, token 8 i + 2 (lane % 4) + t
                     const int nc = nw + 8 * (lane & 3);
 #pragma unroll
-                    for (int g = 0; g < 2; ++g) {   // 16 tokens at a time
-                        __syncwarp();   // the tokens before have left the warp's shared memory
+                    for (int g = 0; g < 2; ++g) {   // 16 tokens at a time, in the two halves in turn
+                        const uint32_t half = turn + 1024u * g;
+                        if (lane == 0) bulk_read_wait<1>();   // the half's last store has read it
+                        __syncwarp();
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
                             const int i = 2 * g + h;
-                            const float2 x2 = *reinterpret_cast<const float2 *>(xs_s + 8 * i + 2 * (lane & 3));
-                            const uint64_t xs2 = f2(x2.x, x2.y);
                             uint32_t o[4];
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
                                 const int at = 16 * (e >> 1) + 4 * i + 2 * (e & 1);
                                 const uint64_t y = finish<GELU>(__float_as_int(v[at]), __float_as_int(v[at + 1]),
-                                                                f2_mul(xs2, f2(wsv[e % NCH], wsv[e % NCH])),
+                                                                f2_mul(xsv[u][i], f2(wsv[e % NCH], wsv[e % NCH])),
                                                                 f2(bv[e % NCH], bv[e % NCH]));
                                 o[e] = pack2<DT>(f2_lo(y), f2_hi(y));
                             }
-                            // transposed into rows of 32 channels: matrix e of the store is channels 8 e .. 8 e + 7
-                            // of tokens 8 i .. 8 i + 7, lane l gives the row of token 8 i + l % 8 of matrix l / 8
+                            // transposed into rows of 32 channels (64-byte swizzle): matrix e of the store is channels
+                            // 8 e .. 8 e + 7 of tokens 8 i .. 8 i + 7, lane l gives the row of token 8 i + l % 8 of
+                            // matrix l / 8
                             const int tok = 8 * h + (lane & 7);
-                            const uint32_t to = turn + (uint32_t)(tok * 64 + (((lane >> 3) ^ ((tok >> 1) & 3)) << 4));
+                            const uint32_t to = half + (uint32_t)(tok * 64 + (((lane >> 3) ^ ((tok >> 1) & 3)) << 4));
                             asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};"
                                          ::"r"(to), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]) : "memory");
                         }
-                        __syncwarp();
-                        // lane l: channels 8 (l % 4) .. + 8 of tokens l / 4 + 8 h
+                        if (p.vec) {
+                            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                            __syncwarp();
+                            if (lane == 0) {   // a group for every half, so that one left is the other half's
+                                if (nw < p.N && 16 * g < rows) tma_store_2d(&tm_out, nw, (int)mc + 16 * g, half);
+                                bulk_commit();
+                            }
+                        } else {   // rows off 16 bytes: lane l stores channels 8 (l % 4) .. + 8 of tokens l / 4 + 8 h
+                            __syncwarp();
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const int at = 8 * h + (lane >> 2), tok = 16 * g + at;
-                            const uint32_t from = turn + (uint32_t)(at * 64 + (((lane & 3) ^ ((at >> 1) & 3)) << 4));
-                            uint4 u;
-                            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                                         : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "r"(from) : "memory");
-                            if (tok < rows) {
+                            for (int h = 0; h < 2; ++h) {
+                                const int at = 8 * h + (lane >> 2), tok = 16 * g + at;
+                                const uint32_t from = half + (uint32_t)(at * 64 + (((lane & 3) ^ ((at >> 1) & 3)) << 4));
+                                uint32_t w4[4];
+                                asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                                             : "=r"(w4[0]), "=r"(w4[1]), "=r"(w4[2]), "=r"(w4[3]) : "r"(from) : "memory");
                                 uint16_t *dst = static_cast<uint16_t *>(p.out) + (mc + tok) * p.out_ld + nc;
-                                if (p.vec && nc + 7 < p.N) {
-                                    *reinterpret_cast<uint4 *>(dst) = u;
-                                } else {
-                                    const uint32_t w4[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-                                    for (int j = 0; j < 8; ++j)
-                                        if (nc + j < p.N) dst[j] = (uint16_t)(w4[j >> 1] >> (16 * (j & 1)));
-                                }
+                                for (int j = 0; j < 8; ++j)
+                                    if (tok < rows && nc + j < p.N) dst[j] = (uint16_t)(w4[j >> 1] >> (16 * (j & 1)));
                             }
                         }
                     }
@@ -396,6 +430,7 @@ kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtenso
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(acc_empty + 8u * (uint32_t)b);
         }
+        if (DT != SS_F32 && lane == 0) bulk_read_wait<0>();   // the shared memory stays until it has been read
         if (!ok) report(p.status, SS_DEV_TIMEOUT);
     } else if (warp == EPI_WARPS) {
         // ---------------- TMA producer (both CTAs) ----------------
@@ -871,8 +906,13 @@ static int launch(const Plan &plan, const int8_t *x, int64_t x_ld, const int8_t 
         if (tiles > 0x7fffffff) return SS_ERR_SHAPE;
         p.ntiles = (int)tiles;
         const int npairs = (int)(tiles < nsm / 2 ? tiles : nsm / 2);
+        CUtensorMap tm_out = {};
+        if (DT != SS_F32 && p.vec) {
+            rc = encode_tmap_2d_b16_sw64(&tm_out, p.out, (uint64_t)p.N, (uint64_t)p.M, (uint64_t)p.out_ld * 2, 32, 16);
+            if (rc) return rc;
+        }
         return (int)launch_after(pair::kernel<DT, GELU>, 2u * (unsigned)npairs, pair::THREADS, pair::SMEM_BYTES, st, 1, tm_w,
-                                 tm_x, p);
+                                 tm_x, tm_out, p);
     }
     p.ncb = (p.N + 127) / 128;
     const unsigned blocks = (unsigned)(p.ncb * ntb * plan.S);

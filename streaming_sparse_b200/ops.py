@@ -132,7 +132,7 @@ class DeviceStatus:
         if bits & DEV_NONFINITE:
             raise FloatingPointError("router produced a non-finite block score")
         if bits & DEV_TIMEOUT:
-            raise RuntimeError("attention kernel pipeline wait timed out")
+            raise RuntimeError("attention or 8-bit linear kernel pipeline wait timed out")
         if bits & DEV_BADID:
             raise IndexError("block id out of range in the attention LUT")
 
