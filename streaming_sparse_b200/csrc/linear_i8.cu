@@ -290,6 +290,8 @@ kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtenso
         for (int tile = pair_id; tile < p.ntiles && ok; tile += npairs, ++it) {
             const int nw = (tile % p.ncb) * 256 + (int)rank * 128 + 32 * (warp & 3);   // the warp's channels
             const int64_t m0 = (int64_t)(tile / p.ncb) * p.tn;
+            // rows that start at 16 bytes leave as TMA boxes, which clip to whole 16 bytes: not those that end inside one
+            const bool boxes = p.vec && (p.N % 8 == 0 || nw + 32 <= p.N);
             // the channels this thread gets of an accumulator: lane (32-bit output), or lane / 4 + 8 i
             float wsv[NCH], bv[NCH];
 #pragma unroll
@@ -401,14 +403,11 @@ kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtenso
                             asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};"
                                          ::"r"(to), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]) : "memory");
                         }
-                        if (p.vec) {
+                        if (boxes) {
                             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                             __syncwarp();
-                            if (lane == 0) {   // a group for every half, so that one left is the other half's
-                                if (nw < p.N && 16 * g < rows) tma_store_2d(&tm_out, nw, (int)mc + 16 * g, half);
-                                bulk_commit();
-                            }
-                        } else {   // rows off 16 bytes: lane l stores channels 8 (l % 4) .. + 8 of tokens l / 4 + 8 h
+                            if (lane == 0 && nw < p.N && 16 * g < rows) tma_store_2d(&tm_out, nw, (int)mc + 16 * g, half);
+                        } else {   // lane l stores channels 8 (l % 4) .. + 8 of tokens l / 4 + 8 h one by one
                             __syncwarp();
 #pragma unroll
                             for (int h = 0; h < 2; ++h) {
@@ -423,6 +422,7 @@ kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtenso
                                     if (tok < rows && nc + j < p.N) dst[j] = (uint16_t)(w4[j >> 1] >> (16 * (j & 1)));
                             }
                         }
+                        if (lane == 0) bulk_commit();   // a group for every half, so that one left is the other half's
                     }
                 }
             }

@@ -240,6 +240,22 @@ def test_linear_i8_strides_and_buffers():
             _between(ref, r, tol)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M", [2, 40, 300, 2000])
+def test_linear_i8_writes_nothing_past_its_columns(M, dtype):
+    """Rows that start at 16 bytes and end inside 16 bytes, at a tile's end and inside one."""
+    for N in (128, 130, 133, 250, 257, 1531, 1539):
+        x, xs = _codes(1, M, 200)
+        w, ws = _codes(2, N, 200)
+        ref = ops.linear_i8(x, xs, w, ws / 300, out_dtype=dtype)
+        for off in (0, 8, 1):
+            buf = torch.full((M + 1, -(-N // 8) * 8 + 16), 7.0, device=DEV, dtype=dtype)
+            out = buf[:M, off:off + N]
+            assert torch.equal(ops.linear_i8(x, xs, w, ws / 300, out=out), ref)
+            out.fill_(7.0)
+            assert (buf == 7.0).all(), (N, off)
+
+
 @pytest.mark.parametrize("M", [1, 6, 20, 130, 2000])
 def test_linear_i8_not_finite_rows(M):
     x, xs, w, ws, b, ref = _check_linear(M, 500, 600, torch.bfloat16, torch.bfloat16, False)
