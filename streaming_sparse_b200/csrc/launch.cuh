@@ -1,4 +1,8 @@
 // launch.cuh -- programmatic dependent launch for kernels that follow one another on a stream.
+//
+// A kernel's own start (barriers, TMEM, descriptors, its blocks' launch) overlaps the end of the kernel
+// before it. Norm, ffn1, quantiser, ffn2 in a CUDA graph on B200, without and with: 16 tokens 17.6 / 15.4 us,
+// 1560 tokens 58.6 / 55.9 us; 4680 x 4608 x 1536 products back to back 29.2 / 27.9 us.
 #pragma once
 
 #include <cuda_runtime.h>

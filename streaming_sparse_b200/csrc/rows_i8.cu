@@ -16,8 +16,8 @@
 // its statistics and its codes. Measured on B200 (bf16, buffers beyond L2; a plain copy reaches 6.54
 // TB/s): quantiser 4680 x 8960 20.4 us (6.2 TB/s), 20000 x 5120 46 us (6.7 TB/s); RMSNorm with the
 // residual's addition 32760 x 1536 53.6 us (6.6 TB/s), 4680 x 1536 10.7 us (4.7 TB/s: two waves of
-// blocks, 6.5 us from L2); AdaLN with the gated addition 32760 x 1536 68.8 us (5.1 TB/s), 4680 x 1536
-// 17.2 us (10.0 us from L2). AdaLN reads three fp32 vectors a row through L1, 18 KB beside the row's own
+// blocks, 6.5 us from L2); AdaLN with the gated addition 32760 x 1536 61.8 us (5.7 TB/s), 4680 x 1536
+// 13.9 us (9.7 us from L2), without it 8.1 us. AdaLN reads three fp32 vectors a row through L1, 18 KB beside the row's own
 // 10.8 KB, and reduces three times: L1's passes and the reductions' chains bound it, not HBM.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -208,6 +208,8 @@ __device__ __forceinline__ void store_codes(int8_t *out, int c, int d, int words
     }
 }
 
+__device__ __forceinline__ void prefetch_l1(const float *p) { asm volatile("prefetch.global.L1 [%0];" ::"l"(p)); }
+
 // The row in registers, NE values a thread: one read of each input, one write of each output. WARP: a
 // warp per row (four rows a block), reductions by shuffles alone; else a block per row, as many threads
 // as its chunks need. Thread t takes chunks t, t + threads, ... of VEC consecutive values, each a single
@@ -241,6 +243,17 @@ __global__ void __launch_bounds__(WARP || NE == 16 ? 128 : NE == 24 ? 1024 : NE 
         if (MODE != QUANT && p.res) {
 #pragma unroll
             for (int i = 0; i < NV; ++i) rv[i].load(r, at(i), d);
+        }
+        // The frame's vectors come to L1 while the row is on its way. Warps of wide 16-bit rows only: AdaLN with the
+        // gated addition, without and with, 4680 x 1536 17.1 / 13.9 us, 32760 x 1536 68.9 / 61.8 us and 32760 x 1024
+        // 48.5 / 46.0 us; slower for 512 values (25.8 / 28.6 us), in blocks (2048 values, 102 / 126 us) and for
+        // fp32 (4680 x 1536 19.5 / 20.2 us).
+        if (MODE == MOD && WARP && NE > 16 && AL && sizeof(T) == 2 && p.gate) {
+            for (int c = (int)threadIdx.x * 32; c < d; c += (int)blockDim.x * 32) {
+                prefetch_l1(p.gate + f * p.gate_ld + c);
+                prefetch_l1(p.scale + f * p.mod_ld + c);
+                prefetch_l1(p.shift + f * p.mod_ld + c);
+            }
         }
 #pragma unroll
         for (int i = 0; i < NV; ++i)
