@@ -140,8 +140,8 @@ __host__ __device__ constexpr int chunk_values() {
     return AL && MODE < MOD ? 16 / (int)sizeof(T) : 4;
 }
 
-// VEC values of a row of d from c on, as loaded: 16 bytes at once (AL, d a multiple of VEC), or one by
-// one; zeros past the row's end (FULL: no chunk lies there)
+// VEC values of a row of d from c on, as loaded: 8 or 16 bytes at once (AL: the chunk lies in the row), or
+// one by one, with zeros past the row's end. FULL: no store lies past it.
 template <typename T, int VEC, bool AL, bool FULL>
 struct Chunk {
     static constexpr int BYTES = VEC * (int)sizeof(T), WORDS = BYTES <= 16 ? 1 : BYTES / 16;
@@ -155,7 +155,7 @@ struct Chunk {
         if constexpr (AL) {
 #pragma unroll
             for (int i = 0; i < WORDS; ++i)
-                u[i] = FULL || c < d ? reinterpret_cast<const Word *>(src + c)[i] : Word{};
+                u[i] = reinterpret_cast<const Word *>(src + c)[i];
         } else {
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
@@ -235,14 +235,19 @@ __global__ void __launch_bounds__(WARP || NE == 16 ? 128 : NE == 24 ? 1024 : NE 
     const T *w = static_cast<const T *>(p.weight), *b = static_cast<const T *>(p.bias);
     const int64_t f = (MODE >= MOD && p.frame_tokens > 0) ? (unsigned)row / (unsigned)p.frame_tokens : 0;
     auto at = [&](int i) { return (i * G + t) * VEC; };
+    // A chunk past the row's end loads the row's last chunk again, which changes no maximum; the sums leave
+    // it out and nothing of it is stored. (Without AL a chunk is filled with zeros past the end.)
+    constexpr bool WHOLE = FULL || !AL;   // every chunk counts
+    auto from = [&](int i) { return WHOLE ? at(i) : min(at(i), d - VEC); };
+    auto in = [&](int i) { return at(i) < d; };
     uint64_t v[NV][VEC / 2];   // pairs of values
     {
         Chunk<T, VEC, AL, FULL> xv[NV], rv[NV];
 #pragma unroll
-        for (int i = 0; i < NV; ++i) xv[i].load(x, at(i), d);
+        for (int i = 0; i < NV; ++i) xv[i].load(x, from(i), d);
         if (MODE != QUANT && p.res) {
 #pragma unroll
-            for (int i = 0; i < NV; ++i) rv[i].load(r, at(i), d);
+            for (int i = 0; i < NV; ++i) rv[i].load(r, from(i), d);
         }
         // The frame's vectors come to L1 while the row is on its way. Warps of wide 16-bit rows only: AdaLN with the
         // gated addition, without and with, 4680 x 1536 17.1 / 13.9 us, 32760 x 1536 68.9 / 61.8 us and 32760 x 1024
@@ -264,7 +269,7 @@ __global__ void __launch_bounds__(WARP || NE == 16 ? 128 : NE == 24 ? 1024 : NE 
 #pragma unroll
                 for (int i = 0; i < NV; ++i) {
                     Chunk<float, VEC, AL, FULL> g;
-                    g.load(p.gate + f * p.gate_ld, at(i), d);
+                    g.load(p.gate + f * p.gate_ld, from(i), d);
 #pragma unroll
                     for (int j = 0; j < VEC / 2; ++j) v[i][j] = add_both(v[i][j], f2_mul(rv[i][j], g[j]));
                 }
@@ -298,50 +303,58 @@ __global__ void __launch_bounds__(WARP || NE == 16 ? 128 : NE == 24 ? 1024 : NE 
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             Chunk<T, VEC, AL, FULL> a;
-            a.load(w, at(i), d);
+            a.load(w, from(i), d);
+            uint64_t part = WHOLE ? s2 : 0ull;
 #pragma unroll
             for (int j = 0; j < VEC / 2; ++j) {
-                s2 = f2_fma(v[i][j], v[i][j], s2);
+                part = f2_fma(v[i][j], v[i][j], part);
                 v[i][j] = f2_mul(v[i][j], a[j]);
                 m = max_abs(max_abs(m, f2_lo(v[i][j])), f2_hi(v[i][j]));
             }
+            if (WHOLE) s2 = part;
+            else if (in(i)) s2 = f2_add(s2, part);
         }
         const float2 a = reduce(f2_lo(s2) + f2_hi(s2), __float_as_uint(m));
         rstd = rsqrtf(__fadd_rn(a.x * p.inv_d, p.eps));
         top = __float_as_uint(a.y);
     } else {
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
+        for (int i = 0; i < NV; ++i) {
+            uint64_t part = WHOLE ? s2 : 0ull;
 #pragma unroll
-            for (int j = 0; j < VEC / 2; ++j) s2 = f2_add(s2, v[i][j]);
+            for (int j = 0; j < VEC / 2; ++j) part = f2_add(part, v[i][j]);
+            if (WHOLE) s2 = part;
+            else if (in(i)) s2 = f2_add(s2, part);
+        }
         const float mean = reduce.sum(f2_lo(s2) + f2_hi(s2)) * p.inv_d;
         s2 = 0ull;
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
+        for (int i = 0; i < NV; ++i) {
+            uint64_t part = WHOLE ? s2 : 0ull;
 #pragma unroll
             for (int j = 0; j < VEC / 2; ++j) {
-                if constexpr (AL) {   // past the row's end v stays 0
-                    if (FULL || at(i) < d) v[i][j] = f2_add(v[i][j], f2(-mean, -mean));
-                } else {
-                    const uint64_t z = f2_add(v[i][j], f2(-mean, -mean));
-                    v[i][j] = f2(at(i) + 2 * j < d ? f2_lo(z) : 0.f, at(i) + 2 * j + 1 < d ? f2_hi(z) : 0.f);
-                }
-                s2 = f2_fma(v[i][j], v[i][j], s2);
+                v[i][j] = f2_add(v[i][j], f2(-mean, -mean));
+                if constexpr (!AL)   // past the row's end
+                    v[i][j] = f2(at(i) + 2 * j < d ? f2_lo(v[i][j]) : 0.f, at(i) + 2 * j + 1 < d ? f2_hi(v[i][j]) : 0.f);
+                part = f2_fma(v[i][j], v[i][j], part);
             }
+            if (WHOLE) s2 = part;
+            else if (in(i)) s2 = f2_add(s2, part);
+        }
         rstd = rsqrtf(__fadd_rn(reduce.sum(f2_lo(s2) + f2_hi(s2)) * p.inv_d, p.eps));
         const uint64_t rstd2 = f2(rstd, rstd);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             if (MODE == AFFINE) {
                 Chunk<T, VEC, AL, FULL> a, e;
-                a.load(w, at(i), d);
-                e.load(b, at(i), d);
+                a.load(w, from(i), d);
+                e.load(b, from(i), d);
 #pragma unroll
                 for (int j = 0; j < VEC / 2; ++j) v[i][j] = f2_fma(v[i][j], f2_mul(rstd2, a[j]), e[j]);
             } else {
                 Chunk<float, VEC, AL, FULL> a, e;
-                a.load(p.scale + f * p.mod_ld, at(i), d);
-                e.load(p.shift + f * p.mod_ld, at(i), d);
+                a.load(p.scale + f * p.mod_ld, from(i), d);
+                e.load(p.shift + f * p.mod_ld, from(i), d);
 #pragma unroll
                 for (int j = 0; j < VEC / 2; ++j) v[i][j] = f2_fma(v[i][j], f2_fma(rstd2, a[j], rstd2), e[j]);
             }
