@@ -235,8 +235,9 @@ __global__ void __launch_bounds__(WARP || NE == 16 ? 128 : NE == 24 ? 1024 : NE 
     const T *w = static_cast<const T *>(p.weight), *b = static_cast<const T *>(p.bias);
     const int64_t f = (MODE >= MOD && p.frame_tokens > 0) ? (unsigned)row / (unsigned)p.frame_tokens : 0;
     auto at = [&](int i) { return (i * G + t) * VEC; };
-    // A chunk past the row's end loads the row's last chunk again, which changes no maximum; the sums leave
-    // it out and nothing of it is stored. (Without AL a chunk is filled with zeros past the end.)
+    // A chunk past the row's end loads the row's last chunk again and counts for nothing: not in the sums, and
+    // not in the maxima either, because the sum stored over an input may have changed what it read. (Without
+    // AL a chunk is filled with zeros past the end.)
     constexpr bool WHOLE = FULL || !AL;   // every chunk counts
     auto from = [&](int i) { return WHOLE ? at(i) : min(at(i), d - VEC); };
     auto in = [&](int i) { return at(i) < d; };
@@ -295,9 +296,13 @@ __global__ void __launch_bounds__(WARP || NE == 16 ? 128 : NE == 24 ? 1024 : NE 
     uint32_t top;
     if (MODE == QUANT) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
+        for (int i = 0; i < NV; ++i) {
+            float most = WHOLE ? m : 0.f;
 #pragma unroll
-            for (int j = 0; j < VEC / 2; ++j) m = max_abs(max_abs(m, f2_lo(v[i][j])), f2_hi(v[i][j]));
+            for (int j = 0; j < VEC / 2; ++j) most = max_abs(max_abs(most, f2_lo(v[i][j])), f2_hi(v[i][j]));
+            if (WHOLE) m = most;
+            else if (in(i)) m = max_abs(m, most);
+        }
         top = reduce.max_bits(__float_as_uint(m));
     } else if (MODE == RMS) {
 #pragma unroll
@@ -305,14 +310,20 @@ __global__ void __launch_bounds__(WARP || NE == 16 ? 128 : NE == 24 ? 1024 : NE 
             Chunk<T, VEC, AL, FULL> a;
             a.load(w, from(i), d);
             uint64_t part = WHOLE ? s2 : 0ull;
+            float most = WHOLE ? m : 0.f;
 #pragma unroll
             for (int j = 0; j < VEC / 2; ++j) {
                 part = f2_fma(v[i][j], v[i][j], part);
                 v[i][j] = f2_mul(v[i][j], a[j]);
-                m = max_abs(max_abs(m, f2_lo(v[i][j])), f2_hi(v[i][j]));
+                most = max_abs(max_abs(most, f2_lo(v[i][j])), f2_hi(v[i][j]));
             }
-            if (WHOLE) s2 = part;
-            else if (in(i)) s2 = f2_add(s2, part);
+            if (WHOLE) {
+                s2 = part;
+                m = most;
+            } else if (in(i)) {
+                s2 = f2_add(s2, part);
+                m = max_abs(m, most);
+            }
         }
         const float2 a = reduce(f2_lo(s2) + f2_hi(s2), __float_as_uint(m));
         rstd = rsqrtf(__fadd_rn(a.x * p.inv_d, p.eps));
@@ -358,8 +369,11 @@ __global__ void __launch_bounds__(WARP || NE == 16 ? 128 : NE == 24 ? 1024 : NE 
 #pragma unroll
                 for (int j = 0; j < VEC / 2; ++j) v[i][j] = f2_fma(v[i][j], f2_fma(rstd2, a[j], rstd2), e[j]);
             }
+            float most = WHOLE ? m : 0.f;
 #pragma unroll
-            for (int j = 0; j < VEC / 2; ++j) m = max_abs(max_abs(m, f2_lo(v[i][j])), f2_hi(v[i][j]));
+            for (int j = 0; j < VEC / 2; ++j) most = max_abs(max_abs(most, f2_lo(v[i][j])), f2_hi(v[i][j]));
+            if (WHOLE) m = most;
+            else if (in(i)) m = max_abs(m, most);
         }
         top = reduce.max_bits(__float_as_uint(m));
     }

@@ -121,6 +121,28 @@ def test_sum_written_over_an_input():
         assert v1 is x and torch.equal(v0, v1) and torch.equal(q0, q1) and torch.equal(s0, s1)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [40, 1400, 1700, 2000, 5000, 8968, 20000, 24584])
+def test_sum_written_over_an_input_at_widths_that_leave_threads_idle(d, dtype):
+    """Threads past the row's end must not see the sum that others store over the inputs: with equal
+    signs a value that is added twice would be the row's largest."""
+    n = 400
+    x, r, w = _rows(1, n, d, dtype).abs(), _rows(2, n, d, dtype).abs(), torch.ones(d, dtype=dtype, device=DEV)
+    b = torch.zeros_like(w)
+    x[:, -8:] += 30
+    em = torch.zeros(1, d, device=DEV)
+    for call in (lambda **kw: ops.rms_norm_i8(kw["a"], w, 1e-6, residual=kw["b"], sum_out=kw.get("to")),
+                 lambda **kw: ops.adaln_i8(kw["a"], eps=1e-6, weight=w, bias=b, y=kw["b"], sum_out=kw.get("to")),
+                 lambda **kw: ops.adaln_i8(kw["a"], eps=1e-6, shift=em, scale=em, frame_tokens=n, y=kw["b"],
+                                           gate=em + 1, sum_out=kw.get("to"))):
+        ref = call(a=x, b=r)
+        for over in ("a", "b"):
+            for _ in range(3):
+                kw = dict(a=x.clone(), b=r.clone())
+                got = call(**kw, to=kw[over])
+                assert all(torch.equal(g, t) for g, t in zip(got, ref))
+
+
 @pytest.mark.parametrize("d", [64, 1536, 1537, 8960, 40000])
 def test_rows_of_zeros_tiny_and_not_finite(d):
     x = _rows(9, 8, d, torch.float32)
