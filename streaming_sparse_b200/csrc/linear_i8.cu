@@ -22,6 +22,7 @@
 
 #include "common.cuh"
 #include "launch.cuh"
+#include "ring.cuh"
 
 namespace ss {
 
@@ -179,29 +180,6 @@ __device__ __forceinline__ bool drain_wait(uint32_t bar, uint32_t parity) {
         if (clock64() - t0 > kWaitLimitCycles) return false;
     return true;
 }
-
-// a place in a ring of n stages and the parity of its barriers there (no division: it is on the
-// critical path of every step)
-struct Ring {
-    int n, at = 0;
-    uint32_t parity = 0;
-    __device__ __forceinline__ void next() {
-        if (++at == n) {
-            at = 0;
-            parity ^= 1u;
-        }
-    }
-    // the j-th stage before this one, j <= n
-    __device__ __forceinline__ Ring before(int j) const {
-        Ring r = *this;
-        r.at -= j;
-        if (r.at < 0) {
-            r.at += n;
-            r.parity ^= 1u;
-        }
-        return r;
-    }
-};
 
 constexpr int BK = 128;                          // codes a stage: one 128-byte swizzled row
 constexpr uint32_t W_BYTES = 128 * BK;           // 128 channels of a stage
@@ -457,14 +435,20 @@ kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtenso
                 issued = min(issued + 1, nst);
             }
         }
+        // The even CTA's tensor core releases the stages of both CTAs by arrivals that nothing orders before the
+        // last accumulator's: they reach this CTA's barriers before its shared memory goes away.
+        if (ok)
+            ok = ring.wait_for_each(issued, [&](int at, uint32_t parity) {
+                return warp_all(mbar_wait(bar(EMPTY + at), parity, abort_flag));
+            });
         if (!ok) report(p.status, SS_DEV_TIMEOUT);
         if (!ok || *abort_flag) {
             // the loads still in flight land before the CTA's shared memory goes away: the even CTA sees
             // both CTAs' by its full barriers, the odd one only by the stages' release
-            for (int j = issued; j > 0; --j) {
-                const Ring r = ring.before(j);
-                drain_wait(bar((rank == 0 ? FULL : EMPTY) + r.at), r.parity);
-            }
+            ring.wait_for_each(issued, [&](int at, uint32_t parity) {
+                drain_wait(bar((rank == 0 ? FULL : EMPTY) + at), parity);
+                return true;
+            });
         }
     } else if (rank == 0) {
         // ---------------- MMA issuer (the even CTA) ----------------
@@ -503,7 +487,7 @@ kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtenso
     }
     tc_fence_before();
     __syncthreads();
-    cluster_sync();   // neither CTA's memory goes away while the other may still signal or read it
+    cluster_sync();   // neither CTA's memory goes away while the other's threads may still signal or read it
     if (warp == 0) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
@@ -595,12 +579,17 @@ kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtenso
             ring.next();
             issued = min(issued + 1, nst);
         }
+        // the stages' last releases reach their barriers before the shared memory goes away
+        if (ok)
+            ok = ring.wait_for_each(issued, [&](int at, uint32_t parity) {
+                return warp_all(mbar_wait(bar(EMPTY + at), parity, abort_flag));
+            });
         if (!ok) report(p.status, SS_DEV_TIMEOUT);
-        if (!ok || *abort_flag)
-            for (int j = issued; j > 0; --j) {   // the loads in flight land before the shared memory goes away
-                const Ring r = ring.before(j);
-                drain_wait(bar(FULL + r.at), r.parity);
-            }
+        if (!ok || *abort_flag)   // the loads in flight land before the shared memory goes away
+            ring.wait_for_each(issued, [&](int at, uint32_t parity) {
+                drain_wait(bar(FULL + at), parity);
+                return true;
+            });
     } else if (warp == 5) {
         const uint32_t idesc = idesc_i8(128, p.tn), bytes = stage_bytes(p.tn);
         const uint64_t dw = smem_desc_sw128(sbase, 16, 1024), dx = smem_desc_sw128(sbase + W_BYTES, 16, 1024);
