@@ -531,6 +531,8 @@ int ss_gate_residual(void *x, const void *y, int64_t y_ld, int n, int d, int fra
 /* lie at any stride (in elements, at least d); `dtype` is SS_BF16, SS_F32 or SS_F16 and holds   */
 /* for x, the residual, the norm's weight and bias, and the stored sum. n may be 0. The kernels    */
 /* start while the one before them on the stream ends, and wait for it before they touch memory.  */
+/* They are launched on the current device, whose memory every pointer and whose stream `stream`   */
+/* has to be.                                                                                     */
 /* ------------------------------------------------------------------------------------------ */
 
 /* q = rint(x * (1 / s)) for rows x [n][d] -> out [n][d] int8, scales [n]. */

@@ -843,7 +843,8 @@ def gate_residual(x: torch.Tensor, y: torch.Tensor, *, gate: torch.Tensor | None
 
 
 # ----------------------------------------------------------------------------------------------
-# 8-bit linear path (csrc/rows_i8.cu, csrc/linear_i8.cu): rows of int8 codes with one scale each
+# 8-bit linear path (csrc/rows_i8.cu, csrc/linear_i8.cu): rows of int8 codes with one scale each.
+# All tensors of a call lie on the current device.
 # ----------------------------------------------------------------------------------------------
 _I8_TYPES = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}   # SS_BF16, SS_F32, SS_F16
 LINEAR_I8_MAX_K = 131071
@@ -855,6 +856,14 @@ def _no_grad(*tensors) -> None:
             if t is not None and t.requires_grad:
                 raise ValueError("the 8-bit linear path has no gradient: call it under torch.no_grad() or detach its "
                                  "inputs")
+
+
+def _check_current(device) -> None:
+    """The library launches on the current device: a stream handle alone (0 for every default stream) does not
+    say which device it is of."""
+    if device.index != torch._C._cuda_getDevice():
+        raise ValueError(f"the tensors are on {device}, which is not the current device: call it under "
+                         f"torch.cuda.device({device.index})")
 
 
 def _stream_handle(device) -> int:
@@ -904,6 +913,7 @@ def rows_i8(n: int, d: int, device) -> torch.Tensor:
 def _rows_i8_in(x: torch.Tensor, name: str):
     if not x.is_cuda or x.dim() != 2 or x.dtype not in _I8_TYPES or x.shape[1] < 1:
         raise ValueError(f"{name}: CUDA tensor [n, d >= 1] of bfloat16, float16 or float32 expected")
+    _check_current(x.device)
     return *x.shape, x.dtype, x.device
 
 
@@ -1033,6 +1043,7 @@ def linear_i8(x_i8: torch.Tensor, xs: torch.Tensor, w_i8: torch.Tensor, ws: torc
     N, dev = w_i8.shape[0], x_i8.device
     if N < 1 or not 1 <= K <= LINEAR_I8_MAX_K:
         raise ValueError(f"N >= 1 and 1 <= K <= {LINEAR_I8_MAX_K} expected, got N = {N}, K = {K}")
+    _check_current(dev)
     _no_grad(xs, ws, bias)
     x_ld, w_ld = _ld(x_i8, "x_i8", M, K, torch.int8, dev), _ld(w_i8, "w_i8", N, K, torch.int8, dev)
     xp, wp = x_i8.data_ptr(), w_i8.data_ptr()

@@ -3,6 +3,7 @@ import ctypes
 
 import pytest
 import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
 
 from streaming_sparse_b200 import ops
 
@@ -61,3 +62,32 @@ def test_rows_i8_start_at_multiples_of_16_bytes():
     for d in (1, 15, 16, 17, 1536, 1549):
         t = ops.rows_i8(3, d, "cpu")
         assert t.shape == (3, d) and t.stride(1) == 1 and t.stride(0) % 16 == 0 and t.stride(0) >= d
+
+
+class NoLibrary:
+    """Stands in for the library: a call that should have been refused before it fails the test."""
+
+    def __getattr__(self, name):
+        def called(*args):
+            pytest.fail(f"{name} was called")
+        return called
+
+
+@pytest.fixture()
+def cuda_tensors(monkeypatch):
+    """CUDA tensors without memory or a GPU, device 0 current, and no library."""
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 0)
+    monkeypatch.setattr(ops, "lib", lambda: NoLibrary())
+    with FakeTensorMode():
+        yield
+
+
+def test_tensors_of_another_device_than_the_current_are_refused(cuda_tensors):
+    dev = torch.device("cuda:1")
+    x, w = torch.empty(4, 64, dtype=torch.bfloat16, device=dev), torch.empty(64, dtype=torch.bfloat16, device=dev)
+    q, s = torch.empty(4, 64, dtype=torch.int8, device=dev), torch.empty(4, device=dev)
+    for call in (lambda: ops.quant_rows(x), lambda: ops.rms_norm_i8(x, w, 1e-6),
+                 lambda: ops.adaln_i8(x, eps=1e-6, weight=w, bias=w), lambda: ops.linear_i8(q, s, q, s)):
+        with pytest.raises(ValueError, match="current device"):
+            call()
