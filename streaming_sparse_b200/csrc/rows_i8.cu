@@ -384,7 +384,8 @@ __global__ void __launch_bounds__(WARP || NE == 16 ? 128 : NE == 24 ? 1024 : NE 
     if (t == 0) p.scales[row] = MODE == RMS ? __fmul_rn(q.s, rstd) : q.s;
 }
 
-// Rows too long for registers: one CTA per row, element loads, the row read once per statistic.
+// Rows too long for registers: one CTA per row, element loads, the row read once per statistic. Places in the
+// row are unsigned: the step past the end of a row of nearly 2^31 values must not wrap to a negative one.
 template <typename T, int MODE>
 __global__ void __launch_bounds__(512) long_row_kernel(const Args p) {
     __shared__ float2 red[2][32];
@@ -392,14 +393,14 @@ __global__ void __launch_bounds__(512) long_row_kernel(const Args p) {
     wait_for_earlier();
     Reduce<false> reduce{red};
     const int64_t row = blockIdx.x;
-    const int t = threadIdx.x, d = p.d;
+    const unsigned t = threadIdx.x, d = (unsigned)p.d;
     const T *x = static_cast<const T *>(p.x) + row * p.x_ld;
     const T *r = p.res ? static_cast<const T *>(p.res) + row * p.res_ld : nullptr;
     const int64_t f = (MODE >= MOD && p.frame_tokens > 0) ? (unsigned)row / (unsigned)p.frame_tokens : 0;
     const float *g = p.gate ? p.gate + f * p.gate_ld : nullptr;
     const T *w = static_cast<const T *>(p.weight), *b = static_cast<const T *>(p.bias);
     const float *sh = p.shift + f * p.mod_ld, *sc = p.scale + f * p.mod_ld;
-    auto value = [&](int c) -> float {
+    auto value = [&](unsigned c) -> float {
         float v = to_f(x[c]);
         if (r) v = __fadd_rn(v, g ? __fmul_rn(to_f(r[c]), g[c]) : to_f(r[c]));
         return v;
@@ -407,32 +408,32 @@ __global__ void __launch_bounds__(512) long_row_kernel(const Args p) {
     float mean = 0.f, rstd = 1.f;
     if (MODE == RMS) {
         float s = 0.f;
-        for (int c = t; c < d; c += blockDim.x) {
+        for (unsigned c = t; c < d; c += blockDim.x) {
             const float v = value(c);
             s += v * v;
         }
         rstd = rsqrtf(__fadd_rn(reduce.sum(s) * p.inv_d, p.eps));
     } else if (MODE >= MOD) {
         float s = 0.f;
-        for (int c = t; c < d; c += blockDim.x) s += value(c);
+        for (unsigned c = t; c < d; c += blockDim.x) s += value(c);
         mean = reduce.sum(s) * p.inv_d;
         s = 0.f;
-        for (int c = t; c < d; c += blockDim.x) {
+        for (unsigned c = t; c < d; c += blockDim.x) {
             const float z = value(c) - mean;
             s += z * z;
         }
         rstd = rsqrtf(__fadd_rn(reduce.sum(s) * p.inv_d, p.eps));
     }
-    auto coded = [&](int c, float v) -> float {   // what the codes stand for, up to RMS's rsqrt
+    auto coded = [&](unsigned c, float v) -> float {   // what the codes stand for, up to RMS's rsqrt
         if (MODE == QUANT) return v;
         if (MODE == RMS) return __fmul_rn(v, to_f(w[c]));
         const float z = (v - mean) * rstd;
         return MODE == AFFINE ? z * to_f(w[c]) + to_f(b[c]) : z * (1.f + sc[c]) + sh[c];
     };
     float m = 0.f;
-    for (int c = t; c < d; c += blockDim.x) m = max_abs(m, coded(c, value(c)));
+    for (unsigned c = t; c < d; c += blockDim.x) m = max_abs(m, coded(c, value(c)));
     const Scale s = row_scale(reduce.max_bits(__float_as_uint(m)));
-    for (int c = t; c < d; c += blockDim.x) {
+    for (unsigned c = t; c < d; c += blockDim.x) {
         const float v = value(c);
         p.out[row * p.out_ld + c] = (int8_t)code(coded(c, v), s);
         // after the last read of x[c] and r[c], by the thread that read them: the sum may be

@@ -320,6 +320,19 @@ def test_offsets_past_32_bits():
         assert torch.equal(out[r:r + 1], ops.linear_i8(x[r:r + 1], xs[r:r + 1], w, ws))
 
 
+def test_the_longest_row():
+    """2^31 - 1 values: the steps past the row's end pass 2^31."""
+    d = 2 ** 31 - 1
+    x = torch.zeros(1, d, dtype=torch.bfloat16, device=DEV)
+    at = torch.tensor([0, 2 ** 30, d - 511, d - 2, d - 1], device=DEV)
+    codes = torch.tensor([1, -2, 50, 3, -127], dtype=torch.int8, device=DEV)
+    x[0, at] = codes.bfloat16()
+    q, s = ops.quant_rows(x)
+    assert s.item() == 1.0 and torch.equal(q[0, at], codes)
+    q[0, at] = 0
+    assert not any(part.any() for part in q[0].split(1 << 28))
+
+
 def test_same_bits_every_time_other_streams_and_graphs():
     x, r, w = _rows(1, 300, 1536, torch.bfloat16), _rows(2, 300, 1536, torch.bfloat16), _rows(3, 1, 1536, torch.bfloat16)[0]
     wq, ws = ops.quant_rows(_rows(4, 520, 1536, torch.bfloat16))
