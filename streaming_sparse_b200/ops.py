@@ -848,6 +848,8 @@ def gate_residual(x: torch.Tensor, y: torch.Tensor, *, gate: torch.Tensor | None
 # ----------------------------------------------------------------------------------------------
 _I8_TYPES = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}   # SS_BF16, SS_F32, SS_F16
 LINEAR_I8_MAX_K = 131071
+LINEAR_I8_MAX_ROWS = 2147480000
+_INT_MAX = 2 ** 31 - 1            # the library takes sizes as 32-bit integers
 
 
 def _no_grad(*tensors) -> None:
@@ -913,6 +915,8 @@ def rows_i8(n: int, d: int, device) -> torch.Tensor:
 def _rows_i8_in(x: torch.Tensor, name: str):
     if not x.is_cuda or x.dim() != 2 or x.dtype not in _I8_TYPES or x.shape[1] < 1:
         raise ValueError(f"{name}: CUDA tensor [n, d >= 1] of bfloat16, float16 or float32 expected")
+    if max(x.shape) > _INT_MAX:
+        raise ValueError(f"{name}: at most {_INT_MAX} rows and values a row expected, got {tuple(x.shape)}")
     _check_current(x.device)
     return *x.shape, x.dtype, x.device
 
@@ -1018,8 +1022,8 @@ def adaln_i8(x: torch.Tensor, *, eps: float, shift: torch.Tensor | None = None, 
         g_ld, gp = _frame_rows(gate, "gate", n, d, frame_tokens, dev), gate.data_ptr()
     r, r_ld, s, sp, s_ld = _residual(y, sum_out, "y", n, d, dtype, dev)
     out, o_ld, scales = _rows_i8_out(out, scales, x, n, d, dev)
-    rc = lib().ss_adaln_i8(x.data_ptr(), x_ld, r, r_ld, gp, g_ld, _I8_TYPES[dtype], n, d, frame_tokens, shp, scp,
-                           mod_ld, wp, bp, eps, sp, s_ld, out.data_ptr(), o_ld, scales.data_ptr(),
+    rc = lib().ss_adaln_i8(x.data_ptr(), x_ld, r, r_ld, gp, g_ld, _I8_TYPES[dtype], n, d, min(frame_tokens, _INT_MAX), shp,
+                           scp, mod_ld, wp, bp, eps, sp, s_ld, out.data_ptr(), o_ld, scales.data_ptr(),
                            _stream_handle(dev))
     if rc:
         check(rc, "ss_adaln_i8")
@@ -1043,6 +1047,8 @@ def linear_i8(x_i8: torch.Tensor, xs: torch.Tensor, w_i8: torch.Tensor, ws: torc
     N, dev = w_i8.shape[0], x_i8.device
     if N < 1 or not 1 <= K <= LINEAR_I8_MAX_K:
         raise ValueError(f"N >= 1 and 1 <= K <= {LINEAR_I8_MAX_K} expected, got N = {N}, K = {K}")
+    if max(M, N) > LINEAR_I8_MAX_ROWS:
+        raise ValueError(f"at most {LINEAR_I8_MAX_ROWS} rows of x_i8 and of w_i8 expected, got {M} and {N}")
     _check_current(dev)
     _no_grad(xs, ws, bias)
     x_ld, w_ld = _ld(x_i8, "x_i8", M, K, torch.int8, dev), _ld(w_i8, "w_i8", N, K, torch.int8, dev)

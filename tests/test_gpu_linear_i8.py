@@ -320,6 +320,15 @@ def test_offsets_past_32_bits():
         assert torch.equal(out[r:r + 1], ops.linear_i8(x[r:r + 1], xs[r:r + 1], w, ws))
 
 
+def test_a_frame_longer_than_32_bits():
+    x = _rows(1, 6, 64, torch.bfloat16)
+    em = 0.3 * torch.randn(1, 2, 64, device=DEV, generator=_gen(7))
+    kw = dict(eps=1e-6, shift=em[:, 0], scale=em[:, 1])
+    for ft in (2 ** 31 - 1, 2 ** 31, 2 ** 32, 2 ** 32 + 1):
+        assert all(torch.equal(a, b) for a, b in zip(ops.adaln_i8(x, frame_tokens=ft, **kw),
+                                                     ops.adaln_i8(x, frame_tokens=6, **kw)))
+
+
 def test_the_longest_row():
     """2^31 - 1 values: the steps past the row's end pass 2^31."""
     d = 2 ** 31 - 1

@@ -91,3 +91,19 @@ def test_tensors_of_another_device_than_the_current_are_refused(cuda_tensors):
                  lambda: ops.adaln_i8(x, eps=1e-6, weight=w, bias=w), lambda: ops.linear_i8(q, s, q, s)):
         with pytest.raises(ValueError, match="current device"):
             call()
+
+
+def test_sizes_past_32_bits_are_refused(cuda_tensors):
+    """The library's sizes are 32-bit integers: larger ones would reach it as their low bits."""
+    dev, big = torch.device("cuda:0"), 2 ** 32 + 64
+    for shape in ((1, big), (big, 1)):
+        x, w = torch.empty(shape, dtype=torch.bfloat16, device=dev), torch.empty(shape[1], dtype=torch.bfloat16, device=dev)
+        for call in (lambda: ops.quant_rows(x), lambda: ops.rms_norm_i8(x, w, 1e-6),
+                     lambda: ops.adaln_i8(x, eps=1e-6, weight=w, bias=w)):
+            with pytest.raises(ValueError, match="at most"):
+                call()
+    q, s = torch.empty(big, 16, dtype=torch.int8, device=dev), torch.empty(big, device=dev)
+    with pytest.raises(ValueError, match="at most"):
+        ops.linear_i8(q, s, q[:8], s[:8])
+    with pytest.raises(ValueError, match="at most"):
+        ops.linear_i8(q[:8], s[:8], q, s)
