@@ -176,19 +176,24 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.Tensor
 # ---------------------------------------------------------------------------------------------
 class Int8Linear:
     """A linear layer on 8-bit rows: its weight as int8 with one scale for each output channel
-    (``ops.quant_rows``, once), applied to 8-bit activations by ``ops.linear_i8``."""
+    (``ops.quant_rows``, once) and a copy of its bias, applied to 8-bit activations by ``ops.linear_i8``."""
 
     def __init__(self, lin: nn.Linear):
-        self.w = self.ws = None
+        self.w = self.ws = self.bias = None
         self.load(lin)
 
     def load(self, lin: nn.Linear) -> None:
-        """Quantise the layer's weight, into the buffers that captured graphs may already read."""
-        w = lin.weight.detach()
+        """Quantise the layer's weight and copy its bias, into the buffers that captured graphs may already
+        read: the layer's own parameters may be replaced meanwhile."""
+        w, b = lin.weight.detach(), lin.bias.detach()
         if self.w is not None and (self.w.shape, self.w.device) != (w.shape, w.device):
-            self.w = self.ws = None
+            self.w = self.ws = self.bias = None
         self.w, self.ws = ops.quant_rows(w, out=self.w, scales=self.ws)
-        self.bias = lin.bias.detach()
+        with torch.inference_mode(False), torch.no_grad():
+            if self.bias is None or self.bias.dtype != b.dtype:
+                self.bias = b.clone()
+            else:
+                self.bias.copy_(b)
 
     def __call__(self, x_i8: torch.Tensor, xs: torch.Tensor, gelu: bool = False) -> torch.Tensor:
         return ops.linear_i8(x_i8, xs, self.w, self.ws, bias=self.bias, gelu=gelu, out_dtype=self.bias.dtype)

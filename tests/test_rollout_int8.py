@@ -89,3 +89,58 @@ def test_int8_is_refused_on_the_host():
     cfg = R.WanConfig(dim=128, ffn_dim=128, num_heads=1, num_layers=1, text_dim=128, text_len=8)
     with pytest.raises(ValueError):
         R.Block(cfg)(torch.zeros(1, 128), None, None, None, None, 0, int8=True)
+
+
+def _replace(lin, factor):
+    lin.weight = torch.nn.Parameter(lin.weight.detach() * factor)
+    lin.bias = torch.nn.Parameter(lin.bias.detach() * factor + 1)
+
+
+def test_loading_again_keeps_the_buffers(monkeypatch):
+    """A captured graph reads the buffers that were there at its capture: they get the new values, and no
+    parameter of the layer is read in their place."""
+    def quant_rows(w, out, scales):   # like the kernel, it writes whatever mode the buffers are from
+        with torch.inference_mode(False), torch.no_grad():
+            out = torch.empty(w.shape, dtype=torch.int8) if out is None else out
+            scales = torch.empty(w.shape[0]) if scales is None else scales
+            scales.copy_(w.abs().amax(1) / 127)
+            return out.copy_(torch.round(w / scales[:, None])), scales
+
+    monkeypatch.setattr(R.ops, "quant_rows", quant_rows)
+    lin = torch.nn.Linear(32, 16)
+    for mode in (torch.no_grad, torch.enable_grad, torch.inference_mode):
+        with mode():
+            layer = R.Int8Linear(lin)
+        kept = layer.w, layer.ws, layer.bias
+        at = [t.data_ptr() for t in kept]
+        old = layer.bias.clone()
+        _replace(lin, 2)
+        assert torch.equal(layer.bias, old)          # until load(), as the weight
+        layer.load(lin)
+        assert [t.data_ptr() for t in (layer.w, layer.ws, layer.bias)] == at
+        assert all(a is b for a, b in zip(kept, (layer.w, layer.ws, layer.bias)))
+        assert torch.equal(layer.bias, lin.bias.detach()) and layer.bias.data_ptr() != lin.bias.data_ptr()
+    layer.load(lin.bfloat16())
+    assert layer.bias.dtype == torch.bfloat16 and torch.equal(layer.bias, lin.bias.detach())
+
+
+@pytest.mark.gpu
+def test_a_captured_layer_reads_what_is_loaded_again():
+    from streaming_sparse_b200 import ops
+
+    dev = _dev()
+    with torch.no_grad():
+        lin = torch.nn.Linear(256, 384, device=dev, dtype=torch.bfloat16)
+        layer = R.Int8Linear(lin)
+        x = ops.quant_rows(torch.randn(70, 256, device=dev, generator=torch.Generator(device=dev).manual_seed(1)))
+        layer(*x)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = layer(*x)
+        _replace(lin, 3)
+        other = [torch.randn(384, device=dev, dtype=torch.bfloat16) for _ in range(8)]   # over memory that was freed
+        layer.load(lin)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, R.Int8Linear(lin)(*x)) and len(other) == 8
