@@ -106,6 +106,32 @@ def test_adaln_i8(n, d, dtype):
         _check_codes(got[0], got[1], o, 127 * tol, tol)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [40, 1536, 1537, 2000, 8960, 20000, 30000])
+def test_sum_without_an_addition(d, dtype):
+    """The C entries store v also where there is nothing to add to x; past the row nothing is written."""
+    from streaming_sparse_b200._lib import lib
+
+    n, kind = 9, ops._I8_TYPES[dtype]
+    x, w, b = _rows(1, n, d, dtype, 8), _rows(2, 1, d, dtype)[0], _rows(3, 1, d, dtype)[0]
+    em = 0.3 * torch.randn(1, 2, d, device=DEV, generator=_gen(7))
+    q, s = ops.rows_i8(n, d, DEV), torch.empty(n, device=DEV)
+    st = torch.cuda.current_stream().cuda_stream
+    to = (q.data_ptr(), q.stride(0), s.data_ptr(), st)
+    for call, want in (
+            (lambda v: lib().ss_rms_norm_i8(x.data_ptr(), d + 8, None, 0, kind, n, d, w.data_ptr(), 1e-6, v, d + 8, *to),
+             ops.rms_norm_i8(x, w, 1e-6)),
+            (lambda v: lib().ss_adaln_i8(x.data_ptr(), d + 8, None, 0, None, 0, kind, n, d, 0, None, None, 0, w.data_ptr(),
+                                         b.data_ptr(), 1e-6, v, d + 8, *to), ops.adaln_i8(x, eps=1e-6, weight=w, bias=b)),
+            (lambda v: lib().ss_adaln_i8(x.data_ptr(), d + 8, None, 0, None, 0, kind, n, d, n, em.data_ptr(),
+                                         em[:, 1].data_ptr(), d, None, None, 1e-6, v, d + 8, *to),
+             ops.adaln_i8(x, eps=1e-6, shift=em[:, 0], scale=em[:, 1], frame_tokens=n))):
+        v = torch.full((n, d + 8), 3.0, dtype=dtype, device=DEV)
+        assert call(v.data_ptr()) == 0
+        assert torch.equal(v[:, :d], x) and (v[:, d:] == 3).all()
+        assert torch.equal(q, want[0]) and torch.equal(s, want[1])
+
+
 def test_sum_written_over_an_input():
     for which in ("x", "residual"):
         x, r, w = _rows(1, 50, 1536, torch.bfloat16), _rows(2, 50, 1536, torch.bfloat16), _rows(3, 1, 1536, torch.bfloat16)[0]
