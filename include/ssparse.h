@@ -541,8 +541,8 @@ int ss_quant_rows(const void *x, int64_t x_ld, int dtype, int n, int d, int8_t *
 
 /* Codes of v * rsqrt(mean(v^2) + eps) * weight, v = x + residual (residual may be NULL: v = x).
  * `sum` (optional) gets v rounded to dtype; it may be x or residual itself. The norm reads v
- * unrounded. The sum of squares is fp32: rows with values above about 1e18 overflow it and get
- * scale 0. */
+ * unrounded. The sum of squares is fp32: a row whose squares overflow it (values above about 1e18)
+ * counts as not finite, codes 0 and scale NaN. */
 int ss_rms_norm_i8(const void *x, int64_t x_ld, const void *residual, int64_t res_ld, int dtype,
                    int n, int d, const void *weight, float eps, void *sum, int64_t sum_ld,
                    int8_t *out, int64_t out_ld, float *scales, void *stream);
@@ -550,8 +550,8 @@ int ss_rms_norm_i8(const void *x, int64_t x_ld, const void *residual, int64_t re
 /* Codes of LayerNorm(v), v = x + y * gate[f] (y NULL: v = x; gate NULL: v = x + y), followed by
  * either the frame's modulation * (1 + scale[f]) + shift[f] or the affine * weight + bias (exactly
  * one of the two forms); f = row / frame_tokens, shift and scale fp32 rows of stride mod_ld, gate
- * fp32 rows of stride gate_ld. frame_tokens counts only where gate, shift or scale is given. `sum`
- * as in ss_rms_norm_i8. */
+ * fp32 rows of stride gate_ld. frame_tokens counts only where gate, shift or scale is given. `sum`,
+ * and rows whose squares overflow, as in ss_rms_norm_i8. */
 int ss_adaln_i8(const void *x, int64_t x_ld, const void *y, int64_t y_ld, const float *gate,
                 int64_t gate_ld, int dtype, int n, int d, int frame_tokens, const float *shift,
                 const float *scale, int64_t mod_ld, const void *weight, const void *bias, float eps,

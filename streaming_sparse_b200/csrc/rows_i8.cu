@@ -9,8 +9,8 @@
 //                   o = z * (1 + scale[f]) + shift[f]  or  z * w + b;
 //                   s = max(max|o| / 127, 1e-30);  q = rint(o * (1 / s))
 // The sum v is also stored, rounded once to the rows' type; the norm reads it unrounded. All
-// statistics are fp32. A row that holds an infinity or a NaN where its codes are made gets codes 0
-// and scale NaN, so that the products it enters are NaN and no other row's are.
+// statistics are fp32. A row that holds an infinity or a NaN where its codes are made, or whose squares'
+// sum overflows fp32, gets codes 0 and scale NaN, so that the products it enters are NaN and no other row's are.
 //
 // Bound: bytes. Each input is read once and each output written once; a row stays in registers between
 // its statistics and its codes. Measured on B200 (bf16, buffers beyond L2; a plain copy reaches 6.54
@@ -86,6 +86,12 @@ __device__ __forceinline__ Scale row_scale(uint32_t m) {
     if (m >= 0x7f800000u) return {__uint_as_float(0x7fc00000u), 0.f, 0u};
     const float s = fmaxf(__fdiv_rn(__uint_as_float(m), 127.f), TINY);
     return {s, __frcp_rn(s), ~0u};
+}
+// 1 / sqrt(mean + eps) of a row's squares. Where their sum overflowed it would be 0 and the row's codes would
+// look like another row's: NaN, so that the row counts as not finite.
+__device__ __forceinline__ float inv_root(float mean, float eps) {
+    const float r = rsqrtf(__fadd_rn(mean, eps));
+    return r > 0.f ? r : __uint_as_float(0x7fc00000u);
 }
 // the code of x is the low byte: adding 1.5 * 2^23 rounds |x| < 2^22 to the nearest integer, ties to even
 constexpr float ROUND = 12582912.f;
@@ -326,8 +332,8 @@ __global__ void __launch_bounds__(WARP || NE == 16 ? 128 : NE == 24 ? 1024 : NE 
             }
         }
         const float2 a = reduce(f2_lo(s2) + f2_hi(s2), __float_as_uint(m));
-        rstd = rsqrtf(__fadd_rn(a.x * p.inv_d, p.eps));
-        top = __float_as_uint(a.y);
+        rstd = inv_root(a.x * p.inv_d, p.eps);
+        top = rstd > 0.f ? __float_as_uint(a.y) : __float_as_uint(rstd);   // the codes are made without it
     } else {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
@@ -352,7 +358,7 @@ __global__ void __launch_bounds__(WARP || NE == 16 ? 128 : NE == 24 ? 1024 : NE 
             if (WHOLE) s2 = part;
             else if (in(i)) s2 = f2_add(s2, part);
         }
-        rstd = rsqrtf(__fadd_rn(reduce.sum(f2_lo(s2) + f2_hi(s2)) * p.inv_d, p.eps));
+        rstd = inv_root(reduce.sum(f2_lo(s2) + f2_hi(s2)) * p.inv_d, p.eps);
         const uint64_t rstd2 = f2(rstd, rstd);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
@@ -412,7 +418,7 @@ __global__ void __launch_bounds__(512) long_row_kernel(const Args p) {
             const float v = value(c);
             s += v * v;
         }
-        rstd = rsqrtf(__fadd_rn(reduce.sum(s) * p.inv_d, p.eps));
+        rstd = inv_root(reduce.sum(s) * p.inv_d, p.eps);
     } else if (MODE >= MOD) {
         float s = 0.f;
         for (unsigned c = t; c < d; c += blockDim.x) s += value(c);
@@ -422,7 +428,7 @@ __global__ void __launch_bounds__(512) long_row_kernel(const Args p) {
             const float z = value(c) - mean;
             s += z * z;
         }
-        rstd = rsqrtf(__fadd_rn(reduce.sum(s) * p.inv_d, p.eps));
+        rstd = inv_root(reduce.sum(s) * p.inv_d, p.eps);
     }
     auto coded = [&](unsigned c, float v) -> float {   // what the codes stand for, up to RMS's rsqrt
         if (MODE == QUANT) return v;
@@ -432,7 +438,9 @@ __global__ void __launch_bounds__(512) long_row_kernel(const Args p) {
     };
     float m = 0.f;
     for (unsigned c = t; c < d; c += blockDim.x) m = max_abs(m, coded(c, value(c)));
-    const Scale s = row_scale(reduce.max_bits(__float_as_uint(m)));
+    uint32_t top = reduce.max_bits(__float_as_uint(m));
+    if (MODE == RMS && !(rstd > 0.f)) top = __float_as_uint(rstd);
+    const Scale s = row_scale(top);
     for (unsigned c = t; c < d; c += blockDim.x) {
         const float v = value(c);
         p.out[row * p.out_ld + c] = (int8_t)code(coded(c, v), s);

@@ -975,7 +975,8 @@ def rms_norm_i8(x: torch.Tensor, weight: torch.Tensor, eps: float, *, residual: 
     x [n, d] bf16, fp16 or fp32 (any row stride), residual like it, weight [d] of the same type.
     v = x + residual in fp32; (x_i8, scales) are the 8-bit rows of v * rsqrt(mean(v^2) + eps) * weight.
     With a residual the sum v, rounded to x's type, is returned third; ``sum_out`` (x or residual
-    themselves, or another buffer) receives it. Non-finite rows as in ``quant_rows``.
+    themselves, or another buffer) receives it. Non-finite rows as in ``quant_rows``; a row whose sum of
+    squares overflows fp32 (values above about 1e18) counts as one.
     """
     n, d, dtype, dev = _rows_i8_in(x, "x")
     _no_grad(x, weight, residual)
@@ -1000,7 +1001,8 @@ def adaln_i8(x: torch.Tensor, *, eps: float, shift: torch.Tensor | None = None, 
     [frames, d], absent: 1), f = row // frame_tokens; (x_i8, scales) are the 8-bit rows of
     LayerNorm(v) * (1 + scale[f]) + shift[f] (fp32 [frames, d], any row stride), or of
     LayerNorm(v) * weight + bias (both [d] of x's type). With y the sum v, rounded to x's type, is
-    returned third; ``sum_out`` (x or y themselves, or another buffer) receives it.
+    returned third; ``sum_out`` (x or y themselves, or another buffer) receives it. Non-finite rows, and
+    rows whose squares overflow, as in ``rms_norm_i8``.
     """
     n, d, dtype, dev = _rows_i8_in(x, "x")
     _no_grad(x, shift, scale, weight, bias, y, gate)

@@ -190,6 +190,30 @@ def test_rows_of_zeros_tiny_and_not_finite(d):
         assert got[1][4:].isfinite().all() and (got[0][6:].abs().amax(1) == 127).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("d", [64, 1000, 1536, 1537, 2048, 8960, 20000, 40000])
+def test_rows_whose_squares_overflow(d, dtype):
+    """Finite rows whose sum of squares is no fp32 number count as not finite; their neighbours are what they were."""
+    x, w, b = _rows(9, 6, d, dtype), _rows(2, 1, d, dtype)[0], _rows(3, 1, d, dtype)[0]
+    em = 0.3 * torch.randn(1, 2, d, device=DEV, generator=_gen(7))
+    big = x.clone()
+    big[1] *= 1e20
+    big[3, d // 2] = 3e19
+    big[4, d - 1] = -1e38
+    keep = torch.tensor([0, 2, 5], device=DEV)
+    for f in (lambda v, **kw: ops.rms_norm_i8(v, w, 1e-6, **kw),
+              lambda v, residual=None: ops.adaln_i8(v, eps=1e-6, weight=w, bias=b, y=residual),
+              lambda v, residual=None: ops.adaln_i8(v, eps=1e-6, shift=em[:, 0], scale=em[:, 1], frame_tokens=6, y=residual)):
+        for kw in ({}, dict(residual=torch.zeros_like(x))):
+            ref, got = f(x, **kw), f(big, **kw)
+            assert got[1][[1, 3, 4]].isnan().all() and not got[0][[1, 3, 4]].any()
+            assert torch.equal(got[0][keep], ref[0][keep]) and torch.equal(got[1][keep], ref[1][keep])
+    # the largest power of two whose d squares sum to less than 2^127 is no overflow
+    x[1] = 2.0 ** int((126.99 - math.log2(d)) / 2)
+    got = ops.rms_norm_i8(x, torch.ones_like(w), 1e-6)
+    assert (got[0][1] == 127).all() and got[1].isfinite().all()
+
+
 def _linear64(x, xs, w, ws, bias, gelu):
     acc = x.double() @ w.double().t()                      # exact: below 2^53
     scaled = acc * xs.double()[:, None] * ws.double()[None, :]
