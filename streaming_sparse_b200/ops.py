@@ -20,6 +20,7 @@ import ctypes
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from ._lib import DEV_BADID, DEV_NONFINITE, DEV_TIMEOUT, check, lib
 
@@ -858,6 +859,10 @@ def _no_grad(*tensors) -> None:
             if t is not None and t.requires_grad:
                 raise ValueError("the 8-bit linear path has no gradient: call it under torch.no_grad() or detach its "
                                  "inputs")
+    if forward_ad._current_level >= 0:   # inside a dual level, which no_grad() does not end
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise ValueError("the 8-bit linear path has no forward-mode gradient: unpack its dual inputs")
 
 
 def _check_current(device) -> None:

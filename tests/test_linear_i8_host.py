@@ -107,3 +107,36 @@ def test_sizes_past_32_bits_are_refused(cuda_tensors):
         ops.linear_i8(q, s, q[:8], s[:8])
     with pytest.raises(ValueError, match="at most"):
         ops.linear_i8(q[:8], s[:8], q, s)
+
+
+def test_tensors_with_a_tangent_are_refused():
+    """Forward-mode derivatives would be lost without a word: under no_grad() too, which does not stop them."""
+    x = torch.randn(4, 8)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        for mode in (torch.enable_grad, torch.no_grad):
+            with mode():
+                with pytest.raises(ValueError, match="forward-mode"):
+                    ops._no_grad(None, x, dual)
+                ops._no_grad(x, None, torch.autograd.forward_ad.unpack_dual(dual).primal)
+    ops._no_grad(x, None)
+    with pytest.raises(ValueError, match="forward-mode"):
+        torch.func.jvp(lambda v: ops._no_grad(v) or v, (x,), (torch.ones_like(x),))
+
+
+@pytest.mark.gpu
+def test_calls_inside_a_dual_level():
+    dev = torch.device("cuda:0")
+    x, w = torch.randn(4, 64, device=dev), torch.ones(64, device=dev)
+    em = torch.randn(1, 2, 64, device=dev)
+    q, s = ops.quant_rows(x)
+    with torch.autograd.forward_ad.dual_level():
+        dual = lambda t: torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))
+        for call in (lambda: ops.quant_rows(dual(x)), lambda: ops.rms_norm_i8(dual(x), w, 1e-6),
+                     lambda: ops.rms_norm_i8(x, dual(w), 1e-6), lambda: ops.rms_norm_i8(x, w, 1e-6, residual=dual(x)),
+                     lambda: ops.adaln_i8(x, eps=1e-6, weight=w, bias=dual(w)),
+                     lambda: ops.adaln_i8(x, eps=1e-6, shift=dual(em[:, 0]), scale=em[:, 1], frame_tokens=4),
+                     lambda: ops.linear_i8(q, dual(s), q, s), lambda: ops.linear_i8(q, s, q, s, bias=dual(s))):
+            with pytest.raises(ValueError, match="forward-mode"):
+                call()
+        assert torch.equal(ops.quant_rows(x)[0], q)
