@@ -85,6 +85,7 @@ extern "C" {
 #define SS_DEV_NONFINITE 0x1    /* a router score was NaN or +-inf */
 #define SS_DEV_TIMEOUT 0x2      /* an mbarrier wait in the attention kernel ran out of budget */
 #define SS_DEV_BADID 0x4        /* a block id in the LUT was out of range */
+#define SS_DEV_LINEAR_TIMEOUT 0x8 /* an mbarrier wait in the 8-bit linear layer ran out of budget */
 
 /* Library version (major*100 + minor). */
 int ss_version(void);
@@ -567,8 +568,8 @@ int ss_adaln_i8(const void *x, int64_t x_ld, const void *y, int64_t y_ld, const 
  * is the tanh form of GELU where gelu != 0, else the identity. x [M][K] and w [N][K] int8, 16-byte
  * aligned with row strides that are multiples of 16 (a row's last 16 bytes may be read whole; what lies
  * past K counts for nothing); bias [N] of bias_dtype or NULL; out [M][N] of
- * out_dtype, row stride out_ld. `status` (optional) gets SS_DEV_TIMEOUT if a wait in the kernel ran
- * out. M may be 0. */
+ * out_dtype, row stride out_ld. `status` (optional) gets SS_DEV_LINEAR_TIMEOUT if a wait in the kernel
+ * ran out. M may be 0. */
 int ss_linear_i8(const int8_t *x, int64_t x_ld, const float *xs, const int8_t *w, int64_t w_ld,
                  const float *ws, const void *bias, int bias_dtype, int gelu, int M, int N, int K,
                  void *out, int64_t out_ld, int out_dtype, int *status, void *stream);

@@ -23,7 +23,7 @@ SS_ERRORS = {
     1006: "cuTensorMapEncodeTiled unavailable or failed",
     1007: "device ordinal beyond the library's 64-device table",
 }
-DEV_NONFINITE, DEV_TIMEOUT, DEV_BADID = 0x1, 0x2, 0x4
+DEV_NONFINITE, DEV_TIMEOUT, DEV_BADID, DEV_LINEAR_TIMEOUT = 0x1, 0x2, 0x4, 0x8
 
 _P, _I, _I64, _F, _SZ = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_size_t
 

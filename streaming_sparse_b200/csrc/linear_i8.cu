@@ -409,7 +409,7 @@ kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtenso
             if (lane == 0) mbar_arrive_cluster(acc_empty + 8u * (uint32_t)b);
         }
         if (DT != SS_F32 && lane == 0) bulk_read_wait<0>();   // the shared memory stays until it has been read
-        if (!ok) report(p.status, SS_DEV_TIMEOUT);
+        if (!ok) report(p.status, SS_DEV_LINEAR_TIMEOUT);
     } else if (warp == EPI_WARPS) {
         // ---------------- TMA producer (both CTAs) ----------------
         const uint32_t x_bytes = (uint32_t)(p.tn / 2) * BK;
@@ -441,7 +441,7 @@ kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtenso
             ok = ring.wait_for_each(issued, [&](int at, uint32_t parity) {
                 return warp_all(mbar_wait(bar(EMPTY + at), parity, abort_flag));
             });
-        if (!ok) report(p.status, SS_DEV_TIMEOUT);
+        if (!ok) report(p.status, SS_DEV_LINEAR_TIMEOUT);
         if (!ok || *abort_flag) {
             // the loads still in flight land before the CTA's shared memory goes away: the even CTA sees
             // both CTAs' by its full barriers, the odd one only by the stages' release
@@ -478,7 +478,7 @@ kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtenso
                 ring.next();
             }
         }
-        if (!ok) report(p.status, SS_DEV_TIMEOUT);
+        if (!ok) report(p.status, SS_DEV_LINEAR_TIMEOUT);
         if (!ok || *abort_flag) {
             if (elect_one()) commit_pair_own(bar(DRAIN));   // arrives once every MMA issued so far is done
             __syncwarp();
@@ -584,7 +584,7 @@ kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtenso
             ok = ring.wait_for_each(issued, [&](int at, uint32_t parity) {
                 return warp_all(mbar_wait(bar(EMPTY + at), parity, abort_flag));
             });
-        if (!ok) report(p.status, SS_DEV_TIMEOUT);
+        if (!ok) report(p.status, SS_DEV_LINEAR_TIMEOUT);
         if (!ok || *abort_flag)   // the loads in flight land before the shared memory goes away
             ring.wait_for_each(issued, [&](int at, uint32_t parity) {
                 drain_wait(bar(FULL + at), parity);
@@ -609,7 +609,7 @@ kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtenso
             __syncwarp();
             ring.next();
         }
-        if (!ok) report(p.status, SS_DEV_TIMEOUT);
+        if (!ok) report(p.status, SS_DEV_LINEAR_TIMEOUT);
         if (!ok || *abort_flag) {
             if (elect_one()) tc_commit(bar(DRAIN));   // arrives once every MMA issued so far is done
             __syncwarp();
@@ -617,7 +617,7 @@ kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtenso
         }
     } else {
         ok = warp_all(mbar_wait(bar(ACC), 0, abort_flag));
-        if (!ok) report(p.status, SS_DEV_TIMEOUT);
+        if (!ok) report(p.status, SS_DEV_LINEAR_TIMEOUT);
         if (ok) {
             tc_fence_after();
             const uint32_t lanes = tmem + ((uint32_t)(32 * warp) << 16);

@@ -22,7 +22,7 @@ import math
 import torch
 from torch.autograd import forward_ad
 
-from ._lib import DEV_BADID, DEV_NONFINITE, DEV_TIMEOUT, check, lib
+from ._lib import DEV_BADID, DEV_LINEAR_TIMEOUT, DEV_NONFINITE, DEV_TIMEOUT, check, lib
 
 HEAD_DIM = 128
 
@@ -133,7 +133,9 @@ class DeviceStatus:
         if bits & DEV_NONFINITE:
             raise FloatingPointError("router produced a non-finite block score")
         if bits & DEV_TIMEOUT:
-            raise RuntimeError("attention or 8-bit linear kernel pipeline wait timed out")
+            raise RuntimeError("attention kernel pipeline wait timed out")
+        if bits & DEV_LINEAR_TIMEOUT:
+            raise RuntimeError("8-bit linear kernel pipeline wait timed out")
         if bits & DEV_BADID:
             raise IndexError("block id out of range in the attention LUT")
 
@@ -1093,4 +1095,4 @@ __all__ = ["Workspace", "DeviceStatus", "route", "router_workspace_bytes", "Rout
            "rows_i8", "quant_rows", "rms_norm_i8", "adaln_i8", "linear_i8"]
 
 # keep the status-bit names importable from here
-DEV_BITS = dict(nonfinite=DEV_NONFINITE, timeout=DEV_TIMEOUT, badid=DEV_BADID)
+DEV_BITS = dict(nonfinite=DEV_NONFINITE, timeout=DEV_TIMEOUT, badid=DEV_BADID, linear_timeout=DEV_LINEAR_TIMEOUT)

@@ -1,5 +1,7 @@
 """The 8-bit linear path without a GPU: what its entry points refuse on the host, and the row layout."""
 import ctypes
+import os
+import re
 
 import pytest
 import torch
@@ -140,3 +142,16 @@ def test_calls_inside_a_dual_level():
             with pytest.raises(ValueError, match="forward-mode"):
                 call()
         assert torch.equal(ops.quant_rows(x)[0], q)
+
+
+def test_a_timeout_says_whose_it_is():
+    for name, text in (("timeout", "attention"), ("linear_timeout", "8-bit linear")):
+        word = ops.DeviceStatus.word("cpu")
+        word.fill_(ops.DEV_BITS[name])
+        with pytest.raises(RuntimeError, match=text) as e:
+            ops.DeviceStatus.check("cpu")
+        assert len([t for t in ("attention", "8-bit linear") if t in str(e.value)]) == 1 and not word.any()
+    assert len(set(ops.DEV_BITS.values())) == len(ops.DEV_BITS)
+    with open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "ssparse.h")) as f:
+        header = {n: int(v, 16) for n, v in re.findall(r"#define SS_DEV_(\w+) (0x\w+)", f.read())}
+    assert header == {n.upper(): v for n, v in ops.DEV_BITS.items()}
