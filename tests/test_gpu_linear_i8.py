@@ -108,6 +108,29 @@ def test_adaln_i8(n, d, dtype):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("d", [40, 1536, 1537, 2000, 8960, 20000, 30000])
+def test_adaln_i8_affine_with_a_gated_addition(d, dtype):
+    """The form between a block's self-attention and its cross-attention: LayerNorm(x + y gate[f]) w + b, its sum over x."""
+    for n, ft, pad in ((1, 1, 0), (13, 5, 0), (24, 8, 3), (300, 100, 8)):
+        x, y = _rows(n + d, n, d, dtype, pad), _rows(n + d + 1, n, d, dtype, pad, 0.5)
+        w, b = _rows(5, 1, d, dtype)[0], _rows(6, 1, d, dtype)[0]
+        em = 0.3 * torch.randn(-(-n // ft), 6, d, device=DEV, generator=_gen(8))
+        f = torch.arange(n, device=DEV) // ft
+        kw = dict(eps=1e-6, weight=w, bias=b, y=y, gate=em[:, 2], frame_tokens=ft)
+        got = ops.adaln_i8(x, **kw)
+        assert torch.equal(got[2], (x.float() + y.float() * em[f, 2]).to(dtype))
+        v = x.double() + y.double() * em[f, 2].double()
+        z = v - v.mean(1, keepdim=True)
+        o = z * torch.rsqrt(z.square().mean(1, keepdim=True) + 1e-6) * w.double() + b.double()
+        tol = 8 * _e(d) + 16 * U   # as in test_adaln_i8
+        _check_codes(got[0], got[1], o, 127 * tol, tol)
+        for over in ("x", "y"):
+            to = (x if over == "x" else y).clone()
+            again = ops.adaln_i8(to if over == "x" else x, **dict(kw, y=to if over == "y" else y), sum_out=to)
+            assert again[2] is to and all(torch.equal(a, c) for a, c in zip(again, got))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [40, 1536, 1537, 2000, 8960, 20000, 30000])
 def test_sum_without_an_addition(d, dtype):
     """The C entries store v also where there is nothing to add to x; past the row nothing is written."""
     from streaming_sparse_b200._lib import lib
@@ -259,6 +282,18 @@ def _check_linear(M, N, K, out_dtype, bias_dtype, gelu, seed=0, **kw):
 def test_linear_i8_small(M, N, K):
     i = M + N + K
     _check_linear(M, N, K, TYPES[i % 3], [None, *TYPES][i % 4], i % 2 == 1, seed=i)
+
+
+@pytest.mark.parametrize("M", [3, 4, 5, 6])
+@pytest.mark.parametrize("N,K", [(1, 1), (5, 3), (64, 64), (1531, 1549), (1536, 1536), (130, 8960), (333, 65000)])
+def test_linear_i8_on_both_sides_of_the_dot_products(M, N, K):
+    """Four tokens are the most of the dot-product kernel; five go to the tensor cores."""
+    for i, dtype in enumerate(TYPES):
+        x, xs, w, ws, b, got = _check_linear(M, N, K, dtype, [None, *TYPES][(i + M) % 4], (i + M) % 2 == 1, seed=M + i)
+        xs = xs.clone()
+        xs[M - 1] = math.nan
+        again = ops.linear_i8(x, xs, w, ws, bias=b, gelu=(i + M) % 2 == 1, out_dtype=dtype)
+        assert again[M - 1].isnan().all() and torch.equal(again[:M - 1], got[:M - 1])
 
 
 @pytest.mark.parametrize("out_dtype", TYPES)
