@@ -7,14 +7,17 @@
 // Integer sums are exact in any order, so how K is split changes no bit of the result.
 //
 // Three kernels: dot products for one to four tokens (weights' bytes), clusters that split K for few
-// tokens (latency), SM pairs for many (L2 and the tensor pipe). Measured on B200 (buffers beyond L2):
-//   one token x 8960 x 1536, GELU          4.1 us, 3.4 TB/s of weights (2.9 us from L2)
+// tokens (latency), SM pairs for many (L2 and the tensor pipe). Measured on B200 (CUDA-graph replay over buffers
+// beyond L2, a fresh process each):
+//   one token x 8960 x 1536, GELU          4.1 us, 3.3 TB/s of weights (2.9 us from L2)
 //   77 x 1531 x 1549 to fp32               6.7 us
-//   4680 x 4608 x 1536                    27.7 us, 2.39 POPS
-//   4680 x 8960 x 1536, GELU              54.9 us, 2.35 POPS (50.7 us without GELU)
-//   4680 x 1536 x 8960 to fp16            44.3 us, 2.91 POPS
-//   32760 x 8960 x 1536, GELU              380 us, 2.37 POPS (power-limited)
-// The library's 8-bit product of these sizes, which stops at the 32-bit sums: 29.7, 54.0, 48.2, 352 us.
+//   4680 x 4608 x 1536                    27.5 us, 2.41 POPS (34.5 us to fp32)
+//   4680 x 8960 x 1536, GELU              54.7 us, 2.35 POPS (50.1 us without GELU)
+//   4680 x 1536 x 1536                    12.7 us, 1.74 POPS
+//   4680 x 1536 x 8960 to fp16            44.8 us, 2.88 POPS
+//   32760 x 8960 x 1536, GELU       354 to 385 us, 2.3 to 2.5 POPS (the clocks fall under load)
+// The library's 8-bit product of these sizes, which stops at the 32-bit sums: 29.8, 54.6, 48.7, 362 us (without the
+// square one).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -194,8 +197,10 @@ constexpr uint32_t W_BYTES = 128 * BK;           // 128 channels of a stage
 //
 // Why pairs: a CTA of its own needs 48 KB a step of 128 x 256 x 128 products, a pair's CTA 32 KB, and L2
 // already delivers 17 TB/s at 256 x 256 (0.277 us a step, 0.27 at the tensor pipe's rate). What
-// bounds it, by leaving parts out: 4680 x 8960 x 1536 takes 51.0 us, 39.9 without the stores of the 84 MB of
-// outputs, 38.0 without the epilogue: the stores, which share L2 with the loads. Eight epilogue warps were
+// bounds it, by leaving parts out: 4680 x 8960 x 1536 takes 50.1 us, 41.1 without the stores of the 84 MB of
+// outputs, 39.1 without the epilogue's arithmetic too, 38.5 without the epilogue: the stores, which share L2 with the
+// loads. With GELU 54.7, 48.4, 39.0 and 38.5 us: its exponentials and reciprocals are not hidden either. 32-bit
+// outputs of 4680 x 4608 x 1536, stored by the warps: 34.5 us, 23.6 without the stores, 20.7 without the epilogue. Eight epilogue warps were
 // latency bound at two a scheduler (54.4 us, 64 with GELU against 56.3). 16-bit outputs leave as TMA boxes of
 // 16 tokens x 32 channels; stored by the warps themselves they took 51.5 us (57 with GELU against 54.9).
 namespace pair {
@@ -502,8 +507,8 @@ kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtenso
 // CTA r of a cluster of S sums its share of K in its tensor memory and lays the sums out in its
 // shared memory as [token][channel]; after a cluster barrier it adds up every S-th part of the
 // tokens over the S CTAs (distributed shared memory) and finishes those rows. Bound by latency: about 4 us
-// to start, load and finish, 0.2 us a step of K, so the split sets the time (16 x 1536 x 8960: 8.0 us over
-// eight CTAs, 13.1 over two).
+// to start, load and finish, 0.2 us a step of K, so the split sets the time (16 x 1536 x 8960: 7.3 us over
+// eight CTAs, 12.1 over two).
 namespace split {
 
 constexpr int THREADS = 192;   // warps 0-3: accumulator rows; 4: TMA; 5: MMA; all: the final rows
@@ -700,8 +705,8 @@ kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtenso
 // The weights are read once, straight to registers, 16 bytes a lane; WPC warps of a block share a
 // group of CH channels, each taking every WPC-th 512 bytes of their rows. Lanes' sums meet by
 // redux, warps' through shared memory. Bytes past K of a row's last 16 count as 0 through x. Bound by
-// the weights' bytes and a launch: 8960 x 1536 weights 4.1 us (floor 2.1), 5.0 with four tokens against 8.8
-// through the tensor cores; with eight tokens it would be 9.2 against 8.8, so four is the limit.
+// the weights' bytes and a launch: 8960 x 1536 weights 4.1 us (floor 2.1), 4.7 with four tokens, where five
+// take 6.6 through the tensor cores; a form for eight tokens took 9.2, so four is the limit.
 namespace dot {
 
 constexpr int WARPS = 8;
@@ -843,10 +848,11 @@ struct Plan {
 
 // Which kernel and tile, by a model of the time in us: a launch, then for each round of tiles the steps
 // over K and the tile's output. The constants are a fit to measured times (both kernels, every tile and
-// split, 5 to 4680 tokens x five weights of 1536 x 1536 to 8960 x 1536 and 1536 x 8960); the plan picked is
-// the fastest measured or within about 10 % of it. What it weighs, at 128 tokens (us): 1536 x 8960 weights, 11.0
-// split over clusters of 8 against 17.5 in pairs, whose steps follow one another; 4608 x 1536, 8.0 in pairs
-// against 8.8 in single CTAs, whose weights are read by twice the CTAs.
+// split, 5 to 4680 tokens x five weights of 1536 x 1536 to 8960 x 1536 and 1536 x 8960; bf16 without GELU, before
+// the kernels started early and stored boxes). As they are now the plan picked is 3 % off the fastest of these on
+// average and 18 % at worst (4096 x 4096 weights, 96 tokens), with fp32 outputs or GELU 3 and 13 %. What it weighs (us):
+// 16 tokens x 1536 x 8960 weights, 7.3 split over clusters of 8 against 16.2 in pairs, whose steps follow one another;
+// 128 tokens x 4608 x 1536, 6.5 in pairs against 7.6 in single CTAs, whose weights are read by twice the CTAs.
 static Plan choose(int M, int N, int K, int nsm) {
     const int npairs = nsm / 2;
     const int64_t ncb2 = (N + 255) / 256, ncb = (N + 127) / 128;

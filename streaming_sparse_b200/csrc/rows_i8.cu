@@ -13,12 +13,17 @@
 // sum overflows fp32, gets codes 0 and scale NaN, so that the products it enters are NaN and no other row's are.
 //
 // Bound: bytes. Each input is read once and each output written once; a row stays in registers between
-// its statistics and its codes. Measured on B200 (bf16, buffers beyond L2; a plain copy reaches 6.54
-// TB/s): quantiser 4680 x 8960 20.4 us (6.2 TB/s), 20000 x 5120 46 us (6.7 TB/s); RMSNorm with the
-// residual's addition 32760 x 1536 53.6 us (6.6 TB/s), 4680 x 1536 10.7 us (4.7 TB/s: two waves of
-// blocks, 6.5 us from L2); AdaLN with the gated addition 32760 x 1536 61.8 us (5.7 TB/s), 4680 x 1536
-// 13.9 us (9.7 us from L2), without it 8.1 us. AdaLN reads three fp32 vectors a row through L1, 18 KB beside the row's own
-// 10.8 KB, and reduces three times: L1's passes and the reductions' chains bound it, not HBM.
+// its statistics and its codes. Measured on B200 (bf16; the inputs', outputs' and codes' bytes over the time of a
+// launch in a CUDA graph of twenty or more over buffers beyond L2, so that but for the last ones' tail the writes
+// are in the time too). In the same way a copy of 32760 x 1536 reaches 6.3 TB/s, an addition (two reads a write)
+// 6.8, of 131040 x 1536 6.6 and 7.0: reads go faster than writes, so what a plain copy reaches is no limit here.
+//   quantiser                        4680 x 8960 20.6 us (6.1 TB/s), 20000 x 5120 44.5 us (6.9)
+//   RMSNorm, residual's addition     32760 x 1536 53.7 us (6.6), 131040 x 1536 204 us (6.9), 4680 x 1536 10.6 us (4.7: two
+//                                    waves of blocks; 6.2 us from L2)
+//   AdaLN, gated addition            32760 x 1536 61 us (5.8), 4680 x 1536 13.7 us (9.5 us from L2); without the gate
+//                                    11.9, affine with it 15.6, without an addition 8.1 us (5.9 us from L2)
+// AdaLN reads three fp32 vectors a row through L1, 18 KB beside the row's own 10.8 KB, and reduces three times: L1's
+// passes and the reductions' chains bound it, not HBM.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 

@@ -1095,4 +1095,5 @@ __all__ = ["Workspace", "DeviceStatus", "route", "router_workspace_bytes", "Rout
            "rows_i8", "quant_rows", "rms_norm_i8", "adaln_i8", "linear_i8"]
 
 # keep the status-bit names importable from here
-DEV_BITS = dict(nonfinite=DEV_NONFINITE, timeout=DEV_TIMEOUT, badid=DEV_BADID, linear_timeout=DEV_LINEAR_TIMEOUT)
+DEV_BITS = dict(nonfinite=DEV_NONFINITE, timeout=DEV_TIMEOUT, badid=DEV_BADID,
+                linear_timeout=DEV_LINEAR_TIMEOUT)

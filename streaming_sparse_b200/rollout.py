@@ -246,7 +246,7 @@ class Block(nn.Module):
         kernels (AdaLN, q/k RMSNorm + RoPE with k/v written into the cache rows, RMSNorm, gated
         residual adds, in place on x); otherwise as the PyTorch expressions below, which state
         the same arithmetic. ``int8`` (fused, after ``quantize_linears``): the linear layers on 8-bit
-        rows, which the norms before them produce together with the residual adds.
+        rows, which the norms before them produce, together with the attentions' residual adds.
         """
         if int8:
             if not (fused and x.is_cuda) or self._i8 is None:
@@ -281,8 +281,9 @@ class Block(nn.Module):
         return x
 
     def _forward_int8(self, x, e0, rope, cache: KVCache, cross, current_start: int):
-        """``_forward_fused`` with every per-token linear layer on 8-bit rows: each norm adds the
-        sublayer before it to the stream and writes the next one's 8-bit input."""
+        """``_forward_fused`` with every per-token linear layer on 8-bit rows: the second and third norms
+        add the attentions' outputs to the stream, and every norm writes the next layer's 8-bit input
+        (the feed-forward's output is added by ``gate_residual``, as there)."""
         cfg, H, lin = self.cfg, self.cfg.num_heads, self._i8
         n, d = x.shape
         ft = n // e0.shape[0]
